@@ -199,6 +199,89 @@ int u15c_kv_append(u15c_stream stream, const void* in, void* pages, const int32_
                    int T, int H, int offset);
 
 /* ------------------------------------------------------------------ */
+/* 8-bit floating point with a scale for each block of 128              */
+/* ------------------------------------------------------------------ */
+
+/* A quantised tensor is q (e4m3, one byte a value, [rows][cols] row-major)
+ * and scale bytes s; it stands for q[r][c] * 2^(s[r][c / 128] - 127). s is
+ * the smallest exponent for which 448 * 2^(s - 127) reaches the largest
+ * magnitude of its block (0 when 2^-118 does), so no finite value saturates;
+ * values are rounded to nearest even, once. A value that is not finite
+ * becomes the NaN code 0x7F and makes every product with its row NaN.
+ * Blocks are 1 x 128 for activations, 128 x 128 for weights (the byte is then
+ * the same for the block's 128 rows); the last block of a row or a column
+ * may be short. cols must be a multiple of 16.
+ *
+ * Scale bytes are packed in 512-byte tiles of 128 rows x 4 blocks. With
+ * G = ceil(cols / 512), the byte of (row r, block b) is at
+ *   ((r / 128) * G + b / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4
+ * in a buffer of u15c_fp8_scale_bytes(rows, cols). Bytes of rows and blocks
+ * that do not exist are neither read nor written. Stacked weights keep each
+ * expert's packed scales apart, one after another. q and scale buffers, and
+ * the bf16 tensors here, must be 16-byte aligned (y, resid and bias of the
+ * products need only their type's alignment). No reference counterpart: the
+ * reference quantises to int8 only. */
+size_t u15c_fp8_scale_bytes(int rows, int cols);
+
+/* x [rows][cols] bf16 -> q, scale, one scale per row and 128 columns. */
+int u15c_quant_rows_fp8(u15c_stream stream, const void* x, uint8_t* q, uint8_t* scale, int rows,
+                        int cols);
+
+/* w [n_experts][N][K] bf16 -> q, scale, one scale per 128 x 128 block of an
+ * expert's matrix. */
+int u15c_quant_weight_fp8(u15c_stream stream, const void* w, uint8_t* q, uint8_t* scale,
+                          int n_experts, int N, int K);
+
+/* y [n_experts][rows][cols] bf16 = what (q, scale) stands for. */
+int u15c_dequant_fp8(u15c_stream stream, const uint8_t* q, const uint8_t* scale, void* y,
+                     int n_experts, int rows, int cols);
+
+/* The residual's addition, the routed RMSNorm and the quantisation in one
+ * pass: s = bf16(x + delta); q, scale = the quantised rows of
+ * s * rsqrt(mean(s^2) + eps) * w_e. delta NULL: s = x. x_out, when non-NULL,
+ * receives s (it may be x or delta). w_stack and segments as
+ * u15c_mot_rms_norm. Feeds u15c_mot_linear_fp8 directly. */
+int u15c_mot_add_rms_norm_quant_fp8(u15c_stream stream, const void* x, const void* delta,
+                                    const void* w_stack, int n_experts, const int* seg_off,
+                                    const int* seg_expert, int nseg, void* x_out, uint8_t* q,
+                                    uint8_t* scale, int rows, int dim, float eps);
+
+/* The routed projection of quantised rows xq [M][K] by quantised weights
+ * wq_stack [n_experts][N][K]; segments as u15c_mot_linear_bf16. Products are
+ * exact, sums f32. epilogue: U15C_EPI_STORE (y = bf16(acc (+ bias))),
+ * U15C_EPI_RESIDUAL (y = bf16(resid + acc), rounded once; y may be resid),
+ * U15C_EPI_SWIGLU (N a multiple of 256, rows interleaved in 128-row blocks
+ * [gate | up]: y [M][N/2] = bf16(silu(gate) * up), rounded once),
+ * U15C_EPI_STORE_F32 (y f32 = acc (+ bias)). M = 0 does nothing. */
+int u15c_mot_linear_fp8(u15c_stream stream, const uint8_t* xq, const uint8_t* sx,
+                        const uint8_t* wq_stack, const uint8_t* sw_stack, int n_experts,
+                        const int* seg_off, const int* seg_expert, int nseg, int epilogue,
+                        const void* bias, const void* resid, void* y, int M, int K, int N);
+
+/* The gate|up projection with a quantised output: (yq [M][N/2], sy) = the
+ * quantised rows of silu(gate) * up, weights as U15C_EPI_SWIGLU. Feeds the
+ * down projection directly. */
+int u15c_mot_swiglu_fp8(u15c_stream stream, const uint8_t* xq, const uint8_t* sx,
+                        const uint8_t* wq_stack, const uint8_t* sw_stack, int n_experts,
+                        const int* seg_off, const int* seg_expert, int nseg, uint8_t* yq,
+                        uint8_t* sy, int M, int K, int N);
+
+/* The gated feed-forward half of a layer, three kernels in a row:
+ *   s = bf16(x + delta) (delta NULL: x), n = quantised RMSNorm(s),
+ *   h = quantised silu(n gate^T) * (n up^T), y = bf16(s + h down^T).
+ * gu [n_experts][2 * inter][hidden] interleaved as U15C_EPI_SWIGLU, down
+ * [n_experts][hidden][inter]; y [rows][hidden] bf16 (it may be x or delta).
+ * ws: u15c_ffn_fp8_workspace_bytes of device memory, 16-byte aligned, owned
+ * by this call until its work on `stream` is done. hidden a multiple of 16,
+ * inter of 128. */
+size_t u15c_ffn_fp8_workspace_bytes(int rows, int hidden, int inter);
+int u15c_mot_ffn_fp8(u15c_stream stream, const void* x, const void* delta,
+                     const void* w_norm_stack, const uint8_t* gu_q, const uint8_t* gu_s,
+                     const uint8_t* down_q, const uint8_t* down_s, int n_experts,
+                     const int* seg_off, const int* seg_expert, int nseg, void* y, void* ws,
+                     int rows, int hidden, int inter, float eps);
+
+/* ------------------------------------------------------------------ */
 /* elementwise (src/u15-metal-ops.h:207-212, 359-370)                   */
 /* ------------------------------------------------------------------ */
 int u15c_swiglu(u15c_stream stream, const void* gate, const void* up, void* y, int rows,

@@ -3,9 +3,11 @@
 // u15_elem.cu. The model half (weights, KV cache, backbone) is in
 // u15_model.cu.
 #include "u15_capi_internal.h"
+#include "u15_fp8.cuh"
 
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 
 namespace u15 {
@@ -261,6 +263,61 @@ int run_gemm(GemmArgs& a, cudaStream_t st)
   return U15C_OK;
 }
 
+namespace {
+// 16-byte accesses and TMA tiles need 16-byte aligned buffers (null passes:
+// the callers say which buffers may be absent)
+bool aligned16(std::initializer_list<const void*> ptrs)
+{
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+  return true;
+}
+}  // namespace
+
+int check_gemm_fp8(const GemmFp8Args& a)
+{
+  if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.n_experts <= 0)
+    return fail(U15C_EINVAL, "gemm_fp8: N, K and n_experts must be positive, M not negative");
+  if (a.K % 16) return fail(U15C_EINVAL, "gemm_fp8: K must be a multiple of 16");
+  if ((long)a.N * a.n_experts > 0x7FFFFFFFL)
+    return fail(U15C_EINVAL, "gemm_fp8: n_experts * N exceeds 2^31 - 1 rows");
+  const bool gu = a.epilogue == kEpiSwiglu || a.epilogue == kEpiSwigluFp8;
+  if (gu && a.N % 256)
+    return fail(U15C_EINVAL,
+                "gemm_fp8: the SwiGLU epilogue needs N (gate+up rows) to be a multiple of 256");
+  // a tensor of no rows may have no address
+  const bool rows_there = a.M == 0 || (a.xq != nullptr && a.sx != nullptr && a.y != nullptr &&
+                                       (a.epilogue != kEpiSwigluFp8 || a.sy != nullptr));
+  if (!rows_there || a.wq == nullptr || a.sw == nullptr)
+    return fail(U15C_EINVAL, "gemm_fp8: null buffer");
+  if (a.epilogue == kEpiResid && a.resid == nullptr && a.M > 0)
+    return fail(U15C_EINVAL, "gemm_fp8: the residual epilogue needs a residual input");
+  if (a.bias != nullptr && a.epilogue != kEpiStore && a.epilogue != kEpiStoreF32)
+    return fail(U15C_EINVAL, "gemm_fp8: a bias goes with the store epilogues only");
+  if (!aligned16({a.xq, a.sx, a.wq, a.sw, a.sy}) ||
+      (a.epilogue == kEpiSwigluFp8 && !aligned16({a.y})))
+    return fail(U15C_EINVAL, "gemm_fp8: quantised tensors and scales must be 16-byte aligned");
+  const int al = a.epilogue == kEpiStoreF32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(a.y) % al || reinterpret_cast<uintptr_t>(a.resid) % 2 ||
+      reinterpret_cast<uintptr_t>(a.bias) % 2)
+    return fail(U15C_EINVAL, "gemm_fp8: y, resid and bias must be aligned to their type");
+  return U15C_OK;
+}
+
+int run_gemm_fp8(GemmFp8Args& a, const SegInfo& seg, cudaStream_t st)
+{
+  const int rc0 = check_gemm_fp8(a);
+  if (rc0) return rc0;
+  if (a.M == 0) return U15C_OK;
+  DevState* d = dev();
+  if (d == nullptr) return U15C_ECUDA;
+  a.dev_err = d->err;
+  a.num_sms = d->sms;
+  std::string err;
+  const int rc = gemm_fp8(a, seg, st, &err);
+  return rc ? fail(rc == 1 ? U15C_EINVAL : U15C_ECUDA, err) : U15C_OK;
+}
+
 }  // namespace u15
 
 using namespace u15;
@@ -477,6 +534,187 @@ int u15c_mot_rms_norm_quant_i8(u15c_stream stream, const void* x, const void* w_
     return fail(U15C_EINVAL, "rms_norm_quant: " + err);
   LAUNCH(launch_rms_norm_quant(x, w_stack, q, scale, rows, dim, eps, seg, ST(stream)),
          "rms_norm_quant");
+}
+
+// ---------------------------------------------------------------- fp8
+size_t u15c_fp8_scale_bytes(int rows, int cols)
+{
+  return rows <= 0 || cols <= 0 ? 0 : (size_t)fp8_scale_bytes(rows, cols);
+}
+
+int u15c_quant_rows_fp8(u15c_stream stream, const void* x, uint8_t* q, uint8_t* scale, int rows,
+                        int cols)
+{
+  if (rows == 0 && cols > 0 && cols % 16 == 0) return U15C_OK;
+  if (x == nullptr || q == nullptr || scale == nullptr || rows < 0 || cols <= 0 || cols % 16 ||
+      !aligned16({x, q, scale}))
+    return fail(U15C_EINVAL, "quant_rows_fp8: null or unaligned buffer, negative rows, or cols not "
+                             "a multiple of 16");
+  LAUNCH(launch_quant_rows_fp8(x, q, scale, rows, cols, ST(stream)), "quant_rows_fp8");
+}
+
+int u15c_quant_weight_fp8(u15c_stream stream, const void* w, uint8_t* q, uint8_t* scale,
+                          int n_experts, int N, int K)
+{
+  if (w == nullptr || q == nullptr || scale == nullptr || n_experts <= 0 || n_experts > 65535 ||
+      N <= 0 || N > 65535 * 128 || K <= 0 || K % 16 || !aligned16({w, q, scale}))
+    return fail(U15C_EINVAL, "quant_weight_fp8: null or unaligned buffer, sizes out of range, or K "
+                             "not a multiple of 16");
+  LAUNCH(launch_quant_weight_fp8(w, q, scale, n_experts, N, K, ST(stream)), "quant_weight_fp8");
+}
+
+int u15c_dequant_fp8(u15c_stream stream, const uint8_t* q, const uint8_t* scale, void* y,
+                     int n_experts, int rows, int cols)
+{
+  if (rows == 0 && n_experts > 0 && cols > 0 && cols % 16 == 0) return U15C_OK;
+  if (q == nullptr || scale == nullptr || y == nullptr || n_experts <= 0 || rows < 0 || cols <= 0 ||
+      cols % 16 || !aligned16({q, scale, y}))
+    return fail(U15C_EINVAL, "dequant_fp8: null or unaligned buffer, sizes out of range, or cols "
+                             "not a multiple of 16");
+  LAUNCH(launch_dequant_fp8(q, scale, y, n_experts, rows, cols, ST(stream)), "dequant_fp8");
+}
+
+int u15c_mot_add_rms_norm_quant_fp8(u15c_stream stream, const void* x, const void* delta,
+                                    const void* w_stack, int n_experts, const int* seg_off,
+                                    const int* seg_expert, int nseg, void* x_out, uint8_t* q,
+                                    uint8_t* scale, int rows, int dim, float eps)
+{
+  const bool bufs = rows == 0 || (x != nullptr && q != nullptr && scale != nullptr);
+  if (!bufs || w_stack == nullptr || n_experts <= 0 || rows < 0 || dim <= 0 || dim % 16 ||
+      !aligned16({x, delta, w_stack, x_out, q, scale}))
+    return fail(U15C_EINVAL, "add_rms_norm_quant_fp8: null or unaligned buffer, sizes out of "
+                             "range, or dim not a multiple of 16");
+  SegInfo seg;
+  std::string err;
+  if (!fill_seg(&seg, seg_off, seg_expert, nseg, rows, n_experts, &err))
+    return fail(U15C_EINVAL, "add_rms_norm_quant_fp8: " + err);
+  if (rows == 0) return U15C_OK;
+  LAUNCH(launch_add_rms_norm_fp8(x, delta, w_stack, x_out, q, scale, rows, dim, eps, seg,
+                                 ST(stream)),
+         "add_rms_norm_quant_fp8");
+}
+
+int u15c_mot_linear_fp8(u15c_stream stream, const uint8_t* xq, const uint8_t* sx,
+                        const uint8_t* wq_stack, const uint8_t* sw_stack, int n_experts,
+                        const int* seg_off, const int* seg_expert, int nseg, int epilogue,
+                        const void* bias, const void* resid, void* y, int M, int K, int N)
+{
+  if (epilogue < U15C_EPI_STORE || epilogue > U15C_EPI_STORE_F32)
+    return fail(U15C_EINVAL, "unknown epilogue");
+  GemmFp8Args a;
+  a.xq = xq;
+  a.sx = sx;
+  a.wq = wq_stack;
+  a.sw = sw_stack;
+  a.n_experts = n_experts;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.epilogue = epilogue;
+  a.bias = bias;
+  a.resid = resid;
+  a.y = y;
+  SegInfo seg;
+  std::string err;
+  if (!fill_seg(&seg, seg_off, seg_expert, nseg, M, n_experts, &err))
+    return fail(U15C_EINVAL, "gemm_fp8: " + err);
+  return run_gemm_fp8(a, seg, ST(stream));
+}
+
+int u15c_mot_swiglu_fp8(u15c_stream stream, const uint8_t* xq, const uint8_t* sx,
+                        const uint8_t* wq_stack, const uint8_t* sw_stack, int n_experts,
+                        const int* seg_off, const int* seg_expert, int nseg, uint8_t* yq,
+                        uint8_t* sy, int M, int K, int N)
+{
+  GemmFp8Args a;
+  a.xq = xq;
+  a.sx = sx;
+  a.wq = wq_stack;
+  a.sw = sw_stack;
+  a.n_experts = n_experts;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.epilogue = kEpiSwigluFp8;
+  a.y = yq;
+  a.sy = sy;
+  SegInfo seg;
+  std::string err;
+  if (!fill_seg(&seg, seg_off, seg_expert, nseg, M, n_experts, &err))
+    return fail(U15C_EINVAL, "gemm_fp8: " + err);
+  return run_gemm_fp8(a, seg, ST(stream));
+}
+
+namespace {
+struct FfnWs {
+  size_t n, ns, h, hs, total;   // byte offsets: normed rows, their scales, SwiGLU rows, scales
+  FfnWs(long rows, int hidden, int inter)
+  {
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    n = 0;
+    ns = up((size_t)rows * hidden);
+    h = ns + up(fp8_scale_bytes(rows, hidden));
+    hs = h + up((size_t)rows * inter);
+    total = hs + up(fp8_scale_bytes(rows, inter));
+  }
+};
+}  // namespace
+
+size_t u15c_ffn_fp8_workspace_bytes(int rows, int hidden, int inter)
+{
+  return rows <= 0 || hidden <= 0 || inter <= 0 ? 0 : FfnWs(rows, hidden, inter).total;
+}
+
+int u15c_mot_ffn_fp8(u15c_stream stream, const void* x, const void* delta,
+                     const void* w_norm_stack, const uint8_t* gu_q, const uint8_t* gu_s,
+                     const uint8_t* down_q, const uint8_t* down_s, int n_experts,
+                     const int* seg_off, const int* seg_expert, int nseg, void* y, void* ws,
+                     int rows, int hidden, int inter, float eps)
+{
+  const bool bufs = rows == 0 || (x != nullptr && y != nullptr && ws != nullptr);
+  if (!bufs || w_norm_stack == nullptr || rows < 0 || n_experts <= 0 || hidden <= 0 ||
+      hidden % 16 || inter <= 0 || inter % 128 || inter > 0x3FFFFFFF ||
+      !aligned16({x, delta, w_norm_stack, y, ws}))
+    return fail(U15C_EINVAL, "ffn_fp8: null or unaligned buffer, negative rows, hidden not a "
+                             "multiple of 16 or inter of 128");
+  SegInfo seg;
+  std::string err;
+  if (!fill_seg(&seg, seg_off, seg_expert, nseg, rows, n_experts, &err))
+    return fail(U15C_EINVAL, "ffn_fp8: " + err);
+  const FfnWs o(rows, hidden, inter);
+  uint8_t* b = static_cast<uint8_t*>(ws);
+  GemmFp8Args up, down;
+  up.xq = b + o.n;
+  up.sx = b + o.ns;
+  up.wq = gu_q;
+  up.sw = gu_s;
+  up.n_experts = n_experts;
+  up.M = rows;
+  up.N = 2 * inter;
+  up.K = hidden;
+  up.epilogue = kEpiSwigluFp8;
+  up.y = b + o.h;
+  up.sy = b + o.hs;
+  down.xq = b + o.h;
+  down.sx = b + o.hs;
+  down.wq = down_q;
+  down.sw = down_s;
+  down.n_experts = n_experts;
+  down.M = rows;
+  down.N = hidden;
+  down.K = inter;
+  down.epilogue = kEpiResid;
+  down.resid = delta != nullptr ? y : x;   // the norm stores s in y
+  down.y = y;
+  int rc = check_gemm_fp8(up);
+  if (!rc) rc = check_gemm_fp8(down);
+  if (rc || rows == 0) return rc;
+  if (dev() == nullptr) return U15C_ECUDA;
+  if (launch_add_rms_norm_fp8(x, delta, w_norm_stack, delta != nullptr ? y : nullptr, b + o.n,
+                              b + o.ns, rows, hidden, eps, seg, ST(stream)))
+    return fail(U15C_ECUDA, "ffn_fp8: norm launch failed");
+  rc = run_gemm_fp8(up, seg, ST(stream));
+  return rc ? rc : run_gemm_fp8(down, seg, ST(stream));
 }
 
 int u15c_split_qk_norm(u15c_stream stream, void* x, const void* w_t, const void* w_hw, int heads,

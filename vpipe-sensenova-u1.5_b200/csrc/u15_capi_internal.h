@@ -67,6 +67,10 @@ int check_attention(int hq, int hkv, int tq, int tk, int mode, int q_offset,
 int run_attention(cudaStream_t st, const void* q, const KvView& kv, void* out, int hq, int hkv,
                   int tq, int tk, int mode, int q_offset, const int32_t* t_index, void* sage_ws);
 int run_gemm(GemmArgs& a, cudaStream_t st);
+// The fp8 products: the checks every entry makes before it launches anything,
+// and the launch.
+int check_gemm_fp8(const GemmFp8Args& a);
+int run_gemm_fp8(GemmFp8Args& a, const SegInfo& seg, cudaStream_t st);
 // The tcgen05 kernel over a paged cache with transposed V pages (the model's
 // layout): every rule, Sage (bidirectional) when sage_ws is non-null. A
 // block-causal call the kernel does not serve (an unaligned t-index vector,

@@ -1,0 +1,79 @@
+// 8-bit floating point (e4m3) with one power-of-two scale per block of 128
+// columns: the scale rule, the packed scale layout and the conversions every
+// fp8 kernel shares.
+//
+// A quantised tensor stands for q[r][c] * 2^(s[r][c / 128] - 127). The scale
+// byte s is the smallest exponent whose 448-fold (e4m3's largest value)
+// reaches the block's largest magnitude, so no finite value saturates. A
+// power of two costs e4m3 nothing in relative precision (only the block's
+// values below 2^-14 of the largest fall under its normal range), multiplies
+// exactly, and is the form the tensor core applies by itself (UE8M0).
+//
+// Scales are packed in 512-byte tiles of 128 rows x 4 blocks, the image of
+// the tensor core's scale columns (32 lanes x 4 columns x 4 bytes): one copy
+// moves a tile to shared memory and one tcgen05.cp from there to TMEM.
+#pragma once
+
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "u15_common.cuh"
+
+namespace u15 {
+
+constexpr int kFp8Block = 128;       // columns (and weight rows) under one scale
+constexpr int kFp8SfTile = 512;      // bytes of a packed tile: 128 rows x 4 blocks
+
+__host__ __device__ __forceinline__ int fp8_blocks(int cols) { return (int)(((long)cols + 127) / 128); }
+__host__ __device__ __forceinline__ int fp8_groups(int cols) { return (int)(((long)cols + 511) / 512); }
+__host__ __device__ __forceinline__ long fp8_scale_bytes(long rows, int cols)
+{
+  return (rows + 127) / 128 * fp8_groups(cols) * kFp8SfTile;
+}
+// byte offset of (row r, block b) in the packed scales of a tensor with `groups`
+__host__ __device__ __forceinline__ long fp8_scale_at(long r, int b, int groups)
+{
+  return ((r >> 7) * groups + (b >> 2)) * kFp8SfTile + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
+}
+
+// The scale byte of a block whose largest magnitude is amax: the smallest s
+// with amax <= 448 * 2^(s - 127), from amax's exponent field and whether its
+// mantissa is above 1.75 (448 = 1.75 * 2^8); 0 for amax below 2^-118.
+__device__ __forceinline__ uint32_t fp8_scale_byte(float amax)
+{
+  const uint32_t u = __float_as_uint(amax);
+  const int s = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return (uint32_t)max(s, 0);
+}
+// 2^(127 - s), a normal float for every s the rule gives (0 .. 248)
+__device__ __forceinline__ float fp8_inv_scale(uint32_t s) { return __uint_as_float((254u - s) << 23); }
+// 2^(s - 127); s = 0 is 2^-127, a subnormal float
+__device__ __forceinline__ float fp8_scale_value(uint32_t s)
+{
+  return s != 0 ? __uint_as_float(s << 23) : __uint_as_float(0x400000u);
+}
+
+// e4m3 codes of v[0..8) * inv as 8 bytes, v[0] lowest: rounded to nearest
+// even. v * 0 is NaN for an Inf (and for a NaN), so a value that is not
+// finite becomes the NaN code instead of saturating to 448.
+__device__ __forceinline__ uint2 fp8_codes8(const float (&v)[8], float inv)
+{
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f;
+    f.x = __fmaf_rn(v[2 * i], 0.0f, v[2 * i] * inv);
+    f.y = __fmaf_rn(v[2 * i + 1], 0.0f, v[2 * i + 1] * inv);
+    h[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+// two e4m3 values as floats (exact)
+__device__ __forceinline__ float2 fp8_pair(uint32_t lo16)
+{
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(lo16 & 0xFFFFu), __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+}  // namespace u15

@@ -63,6 +63,7 @@ enum Epilogue {
   kEpiSwiglu = 2,
   kEpiStoreF32 = 3,
   kEpiTpReduce = 4,   // row-parallel product summed over tensor-parallel ranks (TpPeers)
+  kEpiSwigluFp8 = 5,  // fp8 products only: SwiGLU with a quantised output
 };
 
 // Tensor-parallel peers for the fused row-parallel GEMM (kEpiTpReduce).
@@ -122,6 +123,36 @@ int gemm_tc(const GemmArgs& a, cudaStream_t st, std::string* err);
 // system scope, so the stream's later kernels see the peers' stores.
 int launch_tp_wait(const unsigned long long* done, unsigned long long target, unsigned* err,
                    cudaStream_t st);
+
+// The routed product in 8-bit floating point (u15_gemm_fp8.cu; the format:
+// u15_fp8.cuh). All arguments validated by check_gemm_fp8.
+struct GemmFp8Args {
+  const uint8_t* xq = nullptr;   // [M][K] e4m3
+  const uint8_t* sx = nullptr;   // packed scales
+  const uint8_t* wq = nullptr;   // [n_experts][N][K] e4m3
+  const uint8_t* sw = nullptr;   // packed scales, one tensor per expert
+  int n_experts = 1;
+  int M = 0, N = 0, K = 0;
+  int epilogue = kEpiStore;
+  const void* bias = nullptr;    // bf16 [n_experts][N]
+  const void* resid = nullptr;   // bf16 [M][N]
+  void* y = nullptr;             // bf16 or f32 [M][N]; SwiGLU bf16 or e4m3 [M][N / 2]
+  uint8_t* sy = nullptr;         // kEpiSwigluFp8: y's packed scales
+  unsigned* dev_err = nullptr;
+  int num_sms = 148;
+};
+int gemm_fp8(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err);
+
+// u15_fp8.cu
+int launch_add_rms_norm_fp8(const void* x, const void* delta, const void* w, void* x_out,
+                            uint8_t* q, uint8_t* scale, int rows, int dim, float eps,
+                            const SegInfo& seg, cudaStream_t st);
+int launch_quant_rows_fp8(const void* x, uint8_t* q, uint8_t* scale, int rows, int cols,
+                          cudaStream_t st);
+int launch_quant_weight_fp8(const void* w, uint8_t* q, uint8_t* scale, int n_experts, int N, int K,
+                            cudaStream_t st);
+int launch_dequant_fp8(const uint8_t* q, const uint8_t* scale, void* y, int n_experts, int rows,
+                       int cols, cudaStream_t st);
 
 // Paged or contiguous K/V addressing shared by the attention and KV kernels.
 // Token j of kv head h lives at

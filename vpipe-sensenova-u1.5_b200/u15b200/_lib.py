@@ -86,6 +86,18 @@ SIGNATURES = {
     "u15c_mot_rms_norm": (ip, [vp, vp, vp, ip, i32p, i32p, ip, vp, ip, ip, C.c_float]),
     "u15c_mot_rms_norm_quant_i8": (ip, [vp, vp, vp, ip, i32p, i32p, ip, vp, vp, ip, ip,
                                         C.c_float]),
+    "u15c_fp8_scale_bytes": (C.c_size_t, [ip, ip]),
+    "u15c_quant_rows_fp8": (ip, [vp, vp, vp, vp, ip, ip]),
+    "u15c_quant_weight_fp8": (ip, [vp, vp, vp, vp, ip, ip, ip]),
+    "u15c_dequant_fp8": (ip, [vp, vp, vp, vp, ip, ip, ip]),
+    "u15c_mot_add_rms_norm_quant_fp8": (ip, [vp, vp, vp, vp, ip, i32p, i32p, ip, vp, vp, vp, ip,
+                                             ip, C.c_float]),
+    "u15c_mot_linear_fp8": (ip, [vp, vp, vp, vp, vp, ip, i32p, i32p, ip, ip, vp, vp, vp, ip, ip,
+                                 ip]),
+    "u15c_mot_swiglu_fp8": (ip, [vp, vp, vp, vp, vp, ip, i32p, i32p, ip, vp, vp, ip, ip, ip]),
+    "u15c_ffn_fp8_workspace_bytes": (C.c_size_t, [ip, ip, ip]),
+    "u15c_mot_ffn_fp8": (ip, [vp, vp, vp, vp, vp, vp, vp, vp, ip, i32p, i32p, ip, vp, vp, ip, ip,
+                              ip, C.c_float]),
     "u15c_split_qk_norm": (ip, [vp, vp, vp, vp, ip, ip, ip, C.c_float]),
     "u15c_split_rope": (ip, [vp, vp, vp, vp, ip, ip, ip, ip, ip]),
     "u15c_build_rope_tables": (ip, [vp, vp, vp, vp, ip, ip, ip, ip, C.c_double, C.c_double,
