@@ -76,4 +76,88 @@ __device__ __forceinline__ float2 fp8_pair(uint32_t lo16)
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// ---------------------------------------------------------------------
+// tcgen05 with block scales (kind::mxf8f6f4): D += 2^(sa - 127) 2^(sb - 127) A B^T.
+// The instruction takes one UE8M0 byte a row and 32 columns of K from TMEM: a
+// 32-bit column word holds four bytes, and the instruction descriptor names
+// the byte to use. A word here is the packed tile's: the bytes of four
+// 128-column blocks, so the four K = 32 steps of block b all name byte b % 4,
+// and one copied tile serves 512 columns of K. Row m of an operand is lane
+// m % 32, column m / 32 of its scale columns, in all four lane quadrants.
+// ---------------------------------------------------------------------
+// e4m3 x e4m3, K-major operands, UE8M0 scales: a/b format 0 (e4m3), N >> 3 at
+// bit 17, scale type 1 (UE8M0) at bit 23, M >> 4 at bit 24
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N)
+{
+  return ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
+}
+// the byte of the scale words to use, for B at bit 4 and for A at bit 29
+__device__ __forceinline__ uint32_t idesc_scale_byte(uint32_t id) { return (id << 4) | (id << 29); }
+
+// a packed 512-byte tile in shared memory as 32 rows of 16 bytes: no swizzle,
+// 8-row groups 128 bytes apart
+__device__ __forceinline__ uint64_t smem_desc_sf(uint32_t smem_addr)
+{
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(128 >> 4) << 32;   // SBO
+  d |= (uint64_t)1 << 46;            // version
+  return d;
+}
+// copy such a tile to 4 scale columns (every lane quadrant); MMAs issued
+// after it by the same thread see it, MMAs before it are done with what it
+// overwrites
+__device__ __forceinline__ void sf_copy(uint32_t taddr, uint64_t desc)
+{
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void sf_copy_pair(uint32_t taddr, uint64_t desc)
+{
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                         uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate)
+{
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                              uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                              uint32_t accumulate)
+{
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 3-D tiled load into this CTA's shared memory (no multicast): coordinates
+// (0, group, row block) of the packed scales
+__device__ __forceinline__ void tma_load_sf(uint32_t smem_dst, const CUtensorMap* m, int group,
+                                            int rowblk, uint32_t bar)
+{
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(group), "r"(rowblk), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_sf_pair(uint32_t smem_dst, const CUtensorMap* m, int group,
+                                                 int rowblk, uint32_t bar_cluster)
+{
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(group), "r"(rowblk), "r"(bar_cluster)
+      : "memory");
+}
+
 }  // namespace u15

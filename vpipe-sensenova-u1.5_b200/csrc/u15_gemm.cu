@@ -894,6 +894,27 @@ int make_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols,
   return 0;
 }
 
+int make_tma_fp8_scales(CUtensorMap* out, const void* ptr, uint64_t rowblks, uint64_t groups,
+                        uint32_t box_rowblks, std::string* err)
+{
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    *err = "cuTensorMapEncodeTiled is unavailable (driver too old?)";
+    return 1;
+  }
+  const cuuint64_t dims[3] = {128, groups, rowblks};
+  const cuuint64_t strides[2] = {512, groups * 512};
+  const cuuint32_t box[3] = {128, 1, box_rowblks};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<void*>(ptr), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return 0;
+  *err = "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
+  return 1;
+}
+
 namespace {
 
 template <bool I8, int EPI>

@@ -2,131 +2,501 @@
 //
 //   y[m][n] = epilogue( sum_b 2^(sx[m][b] + sw[n][b] - 254) sum_{k in b} xq[m][k] wq[n][k] )
 //
-// over the blocks b of 128 columns, wq and sw those of row m's expert. This
-// form is the plain one: 16 rows x 128 columns a CTA, products and sums in f32
-// on the FMA pipe, each block's sum scaled as it is added.
+// over the blocks b of 128 columns, wq and sw those of row m's expert, on
+// tcgen05.mma kind::mxf8f6f4, which multiplies in the block scales itself:
+// products exact, sums f32 in TMEM, nothing to rescale on the way.
 #include "u15_fp8.cuh"
 #include "u15_kernels.h"
+
+#include <algorithm>
 
 namespace u15 {
 
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int kRows = 16;
+
+// ---------------------------------------------------------------------
+// Many rows: a CTA pair (tcgen05 cta_group::2) computes 256 x 256 tiles.
+//   warp 0     TMA producer (both CTAs): per stage two k-blocks of 128
+//              columns, 128 rows of A and 128 of B a CTA, and the packed
+//              scale tiles of their group: the CTA's 128 rows of A, all 256 of B
+//   warp 1     MMA issuer (leader): copies the stage's scales to TMEM, then
+//              eight MMAs of K = 32, the block's scale byte in the descriptor
+//   warps 2-9  epilogue, two a TMEM lane quadrant, half the columns each
+// TMEM: two accumulators of 256 columns and the scales need more than 512
+// columns, so the accumulators share 32: tile t + 1's MMAs wait until the
+// epilogue has read those 32 columns of tile t (its first step, ~100 cycles),
+// not the whole tile.
+// ---------------------------------------------------------------------
+constexpr int kKps = 2;                        // k-blocks per stage
+constexpr int kStg = 3;
+constexpr int kTileBytes = 128 * 128;          // one operand, one k-block, one CTA
+constexpr int kStageBytes = 2 * kKps * kTileBytes + 2048;   // operands, then the scales
+constexpr int kSmemPair = kStg * kStageBytes + 1024 /*align*/ + 2048 /*amax*/ + 256 /*bars*/;
+constexpr int kThreadsPair = 320;
+constexpr int kAccStep = 224;                  // accumulator 1 starts 32 columns early
+constexpr int kSfCol = 480;                    // two sets of 4 + 8 scale columns, 16 apart
+
+struct PairParams {
+  int M, N, K;
+  int n_units, n_nblk, n_kblk, n_full;
+  int nseg;
+  int seg_off[kMaxSeg + 1];
+  int seg_expert[kMaxSeg];
+  int unit_start[kMaxSeg + 1];
+  int sf_blk_expert;   // scale row blocks of one expert
+  void* y;
+  const bf16* resid;
+  const bf16* bias;
+  uint8_t* sy;
+  unsigned* err;
+};
+
+struct PairTile {
+  int m0, row_lo, row_hi, expert, nb, half;   // half: -1 full width
+};
+
+__device__ __forceinline__ PairTile pair_tile(const PairParams& p, int t)
+{
+  PairTile r;
+  r.half = -1;
+  if (t >= p.n_full) {
+    const int h = t - p.n_full;
+    t = p.n_full + (h >> 1);
+    r.half = h & 1;
+  }
+  // units (256-row blocks of one segment) run fastest: a round of the
+  // schedule reads few columns of B, and A stays in L2
+  const int unit = t % p.n_units;
+  r.nb = t / p.n_units;
+  int s = 0;
+#pragma unroll 1
+  for (int k = 1; k < p.nseg; ++k)
+    if (unit >= p.unit_start[k]) s = k;
+  r.m0 = (p.seg_off[s] / 256 + (unit - p.unit_start[s])) * 256;
+  r.row_lo = max(r.m0, p.seg_off[s]);
+  r.row_hi = min(r.m0 + 256, p.seg_off[s + 1]);
+  r.expert = p.seg_expert[s];
+  return r;
+}
+
+// silu(g) * u
+__device__ __forceinline__ float swiglu1(float g, float u)
+{
+  return __fdividef(g, 1.0f + expf(-g)) * u;
+}
+
+__device__ __forceinline__ void store32(bf16* dst, const float (&v)[32], int col0, int ncols)
+{
+  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    uint4* d4 = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      d4[q] = make_uint4(pack_bf2(v[q * 8 + 0], v[q * 8 + 1]), pack_bf2(v[q * 8 + 2], v[q * 8 + 3]),
+                         pack_bf2(v[q * 8 + 4], v[q * 8 + 5]), pack_bf2(v[q * 8 + 6], v[q * 8 + 7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (col0 + i < ncols) dst[i] = f2bf(v[i]);
+  }
+}
+__device__ __forceinline__ void store32(float* dst, const float (&v)[32], int col0, int ncols)
+{
+  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      reinterpret_cast<float4*>(dst)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (col0 + i < ncols) dst[i] = v[i];
+  }
+}
+__device__ __forceinline__ void add32(float (&v)[32], const bf16* src, int col0, int ncols)
+{
+  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 u = reinterpret_cast<const uint4*>(src)[q];
+      const float2 a = unpack_bf2(u.x), b = unpack_bf2(u.y), c = unpack_bf2(u.z), d = unpack_bf2(u.w);
+      v[q * 8 + 0] += a.x; v[q * 8 + 1] += a.y; v[q * 8 + 2] += b.x; v[q * 8 + 3] += b.y;
+      v[q * 8 + 4] += c.x; v[q * 8 + 5] += c.y; v[q * 8 + 6] += d.x; v[q * 8 + 7] += d.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (col0 + i < ncols) v[i] += bf2f(src[i]);
+  }
+}
 
 template <int EPI>
-__global__ void __launch_bounds__(256) gemm_fp8_plain_kernel(GemmFp8Args a, SegInfo seg)
+__global__ void __launch_bounds__(kThreadsPair, 1)
+    gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
+                         const __grid_constant__ CUtensorMap tmB,
+                         const __grid_constant__ CUtensorMap tmBh,
+                         const __grid_constant__ CUtensorMap tmSA,
+                         const __grid_constant__ CUtensorMap tmSB,
+                         const __grid_constant__ CUtensorMap tmSBh,
+                         const __grid_constant__ PairParams p)
 {
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
-  __shared__ float sx[kRows][132];
-  __shared__ uint8_t sw[GU ? 2 : 1][128][132];
-  const int s = blockIdx.z, e = seg.expert[s];
-  const int m0 = blockIdx.y * kRows;
-  const int lo = max(m0, seg.off[s]), hi = min(m0 + kRows, seg.off[s + 1]);
-  if (lo >= hi) return;
-  const int n0 = blockIdx.x * (GU ? 256 : 128);
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  const int row = m0 + ty;
-  const bool row_ok = row >= lo && row < hi;
-  const int groups = fp8_groups(a.K), nb = fp8_blocks(a.K);
-  const uint8_t* wq = a.wq + (long)e * a.N * a.K;
-  const uint8_t* ws = a.sw + e * fp8_scale_bytes(a.N, a.K);
-  float acc[2][8] = {};
-  for (int b = 0; b < nb; ++b) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kRows * 128; i += 256) {
-      const int r = i >> 7, c = b * 128 + (i & 127);
-      float v = 0.0f;
-      if (m0 + r >= lo && m0 + r < hi && c < a.K)
-        v = fp8_pair(a.xq[(long)(m0 + r) * a.K + c]).x;
-      sx[r][i & 127] = v;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  float* amax_sm = reinterpret_cast<float*>(smem + kStg * kStageBytes);   // [2 tiles][2 halves][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStg * kStageBytes + 2048);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStg + 8);
+
+  const uint32_t full0 = smem_u32(bars);        // leader: count 2 (one per CTA) + tx
+  const uint32_t empty0 = full0 + 8 * kStg;     // each CTA: leader's multicast commit
+  const uint32_t accf0 = empty0 + 8 * kStg;     // each CTA: leader's multicast commit, per accumulator
+  const uint32_t accr = accf0 + 16;             // leader: 512 epilogue threads, a phase a tile
+  const uint32_t drain = accr + 8;              // each CTA
+  const uint32_t amax0 = drain + 8;             // each CTA: 64 threads a lane quadrant, a phase a tile
+
+  const uint32_t w = warp_id();
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStg; ++s) {
+      mbar_init(full0 + 8 * s, 2);
+      mbar_init(empty0 + 8 * s, 1);
     }
-    for (int i = threadIdx.x; i < (GU ? 2 : 1) * 128 * 128; i += 256) {
-      const int h = i >> 14, r = (i >> 7) & 127, c = b * 128 + (i & 127);
-      const int n = n0 + h * 128 + r;
-      sw[h][r][i & 127] = n < a.N && c < a.K ? wq[(long)n * a.K + c] : 0;
-    }
-    __syncthreads();
-    const float fx = row_ok ? fp8_scale_value(a.sx[fp8_scale_at(row, b, groups)]) : 0.0f;
-    for (int h = 0; h < (GU ? 2 : 1); ++h)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int n = n0 + h * 128 + j * 16 + tx;
-        if (n >= a.N) continue;
-        float t = 0.0f;
-        for (int k = 0; k < 128; k += 2) {
-          const float2 w2 =
-              fp8_pair(*reinterpret_cast<const uint16_t*>(&sw[h][j * 16 + tx][k]));
-          t = __fmaf_rn(sx[ty][k], w2.x, t);
-          t = __fmaf_rn(sx[ty][k + 1], w2.y, t);
+    mbar_init(accf0, 1);
+    mbar_init(accf0 + 8, 1);
+    mbar_init(accr, 512);
+    mbar_init(drain, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(amax0 + 8 * i, 64);
+    fence_barrier_init();
+  }
+  if (w == 0) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSA);
+    tma_prefetch_desc(&tmSB);
+  }
+  tc_fence_before();
+  cluster_sync();   // barriers of both CTAs initialised before any remote arrive
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_launch();
+  griddep_wait();
+
+  const int n_tiles = p.n_full + 2 * (p.n_units * p.n_nblk - p.n_full);
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+
+  if (w == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (lane_id() == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+        const PairTile ti = pair_tile(p, t);
+        const bool half = ti.half >= 0;
+        const int arow = ti.m0 + 128 * (int)rank;
+        const int brow = ti.expert * p.N + ti.nb * 256 + (half ? 128 * ti.half + 64 * (int)rank : 128 * (int)rank);
+        const int sblk = ti.expert * p.sf_blk_expert + ti.nb * 2 + (half ? ti.half : 0);
+        const uint32_t tx = kTileBytes + (half ? kTileBytes / 2 : kTileBytes);
+        const uint32_t tx_sf = half ? 2 * kFp8SfTile : 3 * kFp8SfTile;
+        for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
+          const uint32_t s = it % kStg, ph = (it / kStg) & 1;
+          if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) {
+            ok = false;
+            break;
+          }
+          const int nk = min(kKps, p.n_kblk - kb);
+          const uint32_t fb = mapa_shared(full0 + 8 * s, 0);
+          const uint32_t st = smem_u32(smem) + s * kStageBytes;
+          mbar_arrive_expect_tx_cluster(fb, nk * tx + tx_sf);
+          const uint32_t sf = st + 2 * kKps * kTileBytes;
+          tma_load_sf_pair(sf, &tmSA, kb >> 2, arow >> 7, fb);
+          tma_load_sf_pair(sf + kFp8SfTile, half ? &tmSBh : &tmSB, kb >> 2, sblk, fb);
+          for (int hk = 0; hk < nk; ++hk) {
+            const int kx = (kb + hk) * 128;
+            tma_load_2d_pair(st + hk * kTileBytes, &tmA, kx, arow, fb);
+            tma_load_2d_pair(st + (kKps + hk) * kTileBytes, half ? &tmBh : &tmB, kx, brow, fb);
+          }
         }
-        acc[h][j] += t * fx * fp8_scale_value(ws[fp8_scale_at(n, b, groups)]);
       }
-  }
-  if constexpr (GU) {
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float g = acc[0][j];
-      acc[0][j] = __fdiv_rn(g, 1.0f + expf(-g)) * acc[1][j];
-      m = fmaxf(m, fabsf(acc[0][j]));
+      // unwinding (leader): the last fill of every stage, both CTAs' halves,
+      // has landed once the leader's full barrier for it completes
+      if (leader) {
+        for (uint32_t s = 0; s < kStg; ++s) {
+          if (it > s) {
+            const uint32_t last = ((it - 1 - s) / kStg) * kStg + s;
+            mbar_wait(full0 + 8 * s, (last / kStg) & 1, p.err, kDevWaitDrain);
+          }
+        }
+      }
     }
+  } else if (w == 1) {
+    // ---------------- MMA issuer (leader only) ----------------
+    if (lane_id() == 0) {
+      if (leader) {
+        uint32_t it = 0;
+        int lt = 0;
+        bool ok = true;
+        for (int t = pair; t < n_tiles && ok; t += n_pairs, ++lt) {
+          const bool half = t >= p.n_full;
+          const uint32_t idesc = half ? idesc_e4m3(256, 128) : idesc_e4m3(256, 256);
+          // the previous tile's shared columns have been read (and with them
+          // all of the tile before it)
+          if (lt > 0 && !mbar_wait_cluster_probe(accr, (lt - 1) & 1, p.err, kDevWaitAccEmpty)) break;
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + (lt & 1) * kAccStep;
+          for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
+            const uint32_t s = it % kStg, ph = (it / kStg) & 1;
+            if (!mbar_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const int nk = min(kKps, p.n_kblk - kb);
+            const uint32_t st = smem_u32(smem) + s * kStageBytes;
+            const uint32_t sf = st + 2 * kKps * kTileBytes;
+            const uint32_t sfa = tmem_base + kSfCol + (it & 1) * 16, sfb = sfa + 4;
+            sf_copy_pair(sfa, smem_desc_sf(sf));
+            sf_copy_pair(sfb, smem_desc_sf(sf + kFp8SfTile));
+            if (!half) sf_copy_pair(sfb + 4, smem_desc_sf(sf + 2 * kFp8SfTile));
+            for (int hk = 0; hk < nk; ++hk) {
+              const uint32_t a0 = st + hk * kTileBytes, b0 = st + (kKps + hk) * kTileBytes;
+              const uint32_t id = idesc | idesc_scale_byte((kb + hk) & 3);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t sb = fp8_scale_byte(m);
-    const float inv = fp8_inv_scale(sb);
-    if (!row_ok) return;
-    const int nout = a.N / 2;
+              for (int k = 0; k < 4; ++k)
+                mma_e4m3_pair(d_tmem, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), id,
+                              sfa, sfb, ((kb + hk) | k) != 0);
+            }
+            mma_commit_pair_mc(empty0 + 8 * s, 0x3);
+          }
+          if (!ok) break;
+          mma_commit_pair_mc(accf0 + 8 * (lt & 1), 0x3);
+        }
+        mma_commit_pair_mc(drain, 0x3);
+      }
+      // both CTAs: every MMA that writes this CTA's TMEM has completed
+      mbar_wait(drain, 0, p.err, kDevWaitDrain);
+    }
+  } else {
+    // ---------------- epilogue (warps 2..9, both CTAs) ----------------
+    const int wq = (int)(w & 3), wh = (int)(w - 2) >> 2;   // lane quadrant, half of the columns
+    const int r_in = wq * 32 + (int)lane_id();
+    const uint32_t accr_leader = mapa_shared(accr, 0);
+    int lt = 0;
+    for (int t = pair; t < n_tiles; t += n_pairs, ++lt) {
+      const PairTile ti = pair_tile(p, t);
+      const bool half = ti.half >= 0;
+      const int acc = lt & 1;
+      if (!mbar_wait(accf0 + 8 * acc, (lt >> 1) & 1, p.err, kDevWaitAccFull)) break;
+      tc_fence_after();
+      const int row = ti.m0 + 128 * (int)rank + r_in;
+      const bool row_ok = row >= ti.row_lo && row < ti.row_hi;
+      const uint32_t tb = tmem_base + acc * kAccStep + ((uint32_t)(wq * 32) << 16);
+      // the 32 columns the accumulators share are the last of accumulator 0
+      // and the first of accumulator 1; their warps read them first
+      const bool shared_here = wh == (acc ^ 1);
+      bool released = false;
+      auto release = [&] {
+        if (released) return;
+        released = true;
+        tc_fence_before();
+        mbar_arrive_cluster(accr_leader);
+      };
+      if (!shared_here) release();
+      if constexpr (GU) {
+        // columns [0, 128) are gate rows, [128, 256) the matching up rows;
+        // this warp's 64 outputs in two runs of 32, the shared columns' first
+        const int nout = p.N / 2;
+        float h[2][32];
+        int run[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = blockIdx.x * 128 + j * 16 + tx;
-      if constexpr (EPI == kEpiSwiglu) {
-        static_cast<bf16*>(a.y)[(long)row * nout + c] = f2bf(acc[0][j]);
+        for (int i = 0; i < 2; ++i) {
+          run[i] = wh * 2 + (acc == 0 && wh == 1 ? 1 - i : i);
+          uint32_t g[32], u[32];
+          tmem_ld32(tb + run[i] * 32, g);
+          tmem_ld32(tb + 128 + run[i] * 32, u);
+          tmem_ld_wait();
+          release();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            h[i][j] = swiglu1(__uint_as_float(g[j]), __uint_as_float(u[j]));
+        }
+        if constexpr (EPI == kEpiSwiglu) {
+          bf16* yrow = static_cast<bf16*>(p.y) + (long)row * nout + ti.nb * 128;
+          if (row_ok) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              store32(yrow + run[i] * 32, h[i], ti.nb * 128 + run[i] * 32, nout);
+          }
+        } else {
+          // the row's largest of 128 outputs, over the quadrant's two warps
+          float m = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) m = fmaxf(m, fabsf(h[i][j]));
+          float* am = amax_sm + acc * 256;
+          am[wh * 128 + r_in] = m;
+          mbar_arrive(amax0 + 8 * wq);
+          if (!mbar_wait(amax0 + 8 * wq, lt & 1, p.err, kDevWaitAccFull)) break;
+          m = fmaxf(m, am[(wh ^ 1) * 128 + r_in]);
+          const uint32_t sb = fp8_scale_byte(m);
+          const float inv = fp8_inv_scale(sb);
+          if (row_ok) {
+            uint8_t* yrow = static_cast<uint8_t*>(p.y) + (long)row * nout + ti.nb * 128;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint2 c[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = h[i][q * 8 + j];
+                c[q] = fp8_codes8(v, inv);
+              }
+              uint4* d = reinterpret_cast<uint4*>(yrow + run[i] * 32);
+              d[0] = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
+              d[1] = make_uint4(c[2].x, c[2].y, c[3].x, c[3].y);
+            }
+            if (wh == 0) p.sy[fp8_scale_at(row, ti.nb, fp8_groups(nout))] = (uint8_t)sb;
+          }
+        }
       } else {
-        const float v = __fmaf_rn(acc[0][j], 0.0f, acc[0][j] * inv);
-        static_cast<uint8_t*>(a.y)[(long)row * nout + c] =
-            __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+        const int n0 = ti.nb * 256 + (half ? 128 * ti.half : 0);
+        const int nch = half ? 2 : 4;                 // chunks of 32 columns of this warp
+        const int first = half ? wh * 2 : wh * 4;
+        // a half-width tile uses columns [0, 128) of its accumulator: only
+        // accumulator 1 shares any of them
+        const int lead = acc == 0 && !half && wh == 1 ? 3 : 0;
+        if (half && acc == 0) release();
+#pragma unroll 1
+        for (int i = 0; i < nch; ++i) {
+          const int c = first + ((i + lead) & (nch - 1));
+          uint32_t r[32];
+          tmem_ld32(tb + c * 32, r);
+          tmem_ld_wait();
+          release();
+          const int col0 = n0 + c * 32;
+          if (!row_ok || col0 >= p.N) continue;
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          if (p.bias != nullptr) add32(v, p.bias + (long)ti.expert * p.N + col0, col0, p.N);
+          if constexpr (EPI == kEpiResid) add32(v, p.resid + (long)row * p.N + col0, col0, p.N);
+          if constexpr (EPI == kEpiStoreF32)
+            store32(static_cast<float*>(p.y) + (long)row * p.N + col0, v, col0, p.N);
+          else
+            store32(static_cast<bf16*>(p.y) + (long)row * p.N + col0, v, col0, p.N);
+        }
       }
     }
-    if (EPI == kEpiSwigluFp8 && tx == 0)
-      a.sy[fp8_scale_at(row, blockIdx.x, fp8_groups(nout))] = (uint8_t)sb;
-    return;
   }
-  if (!row_ok) return;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int n = n0 + j * 16 + tx;
-    if (n >= a.N) continue;
-    float v = acc[0][j];
-    const long at = (long)row * a.N + n;
-    if (a.bias != nullptr) v += bf2f(static_cast<const bf16*>(a.bias)[(long)e * a.N + n]);
-    if (EPI == kEpiResid) v += bf2f(static_cast<const bf16*>(a.resid)[at]);
-    if (EPI == kEpiStoreF32)
-      static_cast<float*>(a.y)[at] = v;
-    else
-      static_cast<bf16*>(a.y)[at] = f2bf(v);
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the peer's smem and TMEM stay alive until the pair is done
+  if (w == 0) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
   }
+}
+
+// Persistent grid: as many pairs as can be resident at once (not every SM has
+// a usable partner).
+template <int EPI>
+int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+{
+  static std::atomic<uint64_t> attr_set;
+  static std::atomic<int> max_pairs_dev[64];   // resident pairs, per device (0: not yet known)
+  constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
+  PairParams p{};
+  p.M = a.M;
+  p.N = a.N;
+  p.K = a.K;
+  p.y = a.y;
+  p.resid = static_cast<const bf16*>(a.resid);
+  p.bias = static_cast<const bf16*>(a.bias);
+  p.sy = a.sy;
+  p.err = a.dev_err;
+  p.nseg = seg.nseg;
+  for (int s = 0; s < seg.nseg; ++s) {
+    p.seg_off[s] = seg.off[s];
+    p.seg_expert[s] = seg.expert[s];
+    p.unit_start[s] = p.n_units;
+    if (seg.off[s + 1] > seg.off[s])
+      p.n_units += (seg.off[s + 1] + 255) / 256 - seg.off[s] / 256;
+  }
+  p.seg_off[seg.nseg] = seg.off[seg.nseg];
+  p.unit_start[seg.nseg] = p.n_units;
+  p.n_nblk = (a.N + 255) / 256;
+  p.n_kblk = fp8_blocks(a.K);
+  p.sf_blk_expert = (a.N + 127) / 128;
+  if ((long)p.n_units * p.n_nblk > 0x3FFFFFFFL) {
+    *err = "gemm_fp8: too many output tiles";
+    return 1;
+  }
+  CUtensorMap ma, mb, mbh, msa, msb, msbh;
+  const uint64_t wrows = (uint64_t)a.N * a.n_experts, groups = fp8_groups(a.K),
+                 wblks = (uint64_t)p.sf_blk_expert * a.n_experts, xblks = (a.M + 127) / 128;
+  if (make_tma_2d(&ma, a.xq, a.M, a.K, 128, 1, err) || make_tma_2d(&mb, a.wq, wrows, a.K, 128, 1, err) ||
+      make_tma_2d(&mbh, a.wq, wrows, a.K, 64, 1, err) ||
+      make_tma_fp8_scales(&msa, a.sx, xblks, groups, 1, err) ||
+      make_tma_fp8_scales(&msb, a.sw, wblks, groups, 2, err) ||
+      make_tma_fp8_scales(&msbh, a.sw, wblks, groups, 1, err))
+    return 2;
+  auto k = gemm_fp8_pair_kernel<EPI>;
+  if (!smem_attr_once(k, kSmemPair, attr_set)) return 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreadsPair);
+  cfg.dynamicSmemBytes = kSmemPair;
+  cfg.stream = st;
+  cudaLaunchAttribute attrs[2] = {};
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = 2;
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = 1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 2;
+  int max_pairs = max_pairs_dev[dev & 63].load(std::memory_order_relaxed);
+  if (max_pairs <= 0) {
+    cfg.gridDim = dim3(2);
+    if (cudaOccupancyMaxActiveClusters(&max_pairs, k, &cfg) != cudaSuccess || max_pairs <= 0)
+      max_pairs = 64;
+    max_pairs_dev[dev & 63].store(max_pairs, std::memory_order_relaxed);
+  }
+  // a last round that would leave at least half the pairs idle runs as
+  // half-width tiles (a SwiGLU tile holds whole gate and up blocks: it is not
+  // split)
+  const int tiles = p.n_units * p.n_nblk, pairs = std::min(tiles, max_pairs), rest = tiles % pairs;
+  p.n_full = !GU && rest > 0 && 2 * rest <= pairs ? tiles - rest : tiles;
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, ma, mb, mbh, msa, msb, msbh, p) == cudaSuccess ? 0 : 2;
 }
 
 }  // namespace
 
 int gemm_fp8(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
 {
-  if (a.M <= 0) return 0;
-  const bool gu = a.epilogue == kEpiSwiglu || a.epilogue == kEpiSwigluFp8;
-  const dim3 grid((a.N + (gu ? 255 : 127)) / (gu ? 256 : 128), (a.M + kRows - 1) / kRows, seg.nseg);
+  err->clear();
+  int rc;
   switch (a.epilogue) {
-    case kEpiStore: gemm_fp8_plain_kernel<kEpiStore><<<grid, 256, 0, st>>>(a, seg); break;
-    case kEpiResid: gemm_fp8_plain_kernel<kEpiResid><<<grid, 256, 0, st>>>(a, seg); break;
-    case kEpiSwiglu: gemm_fp8_plain_kernel<kEpiSwiglu><<<grid, 256, 0, st>>>(a, seg); break;
-    case kEpiStoreF32: gemm_fp8_plain_kernel<kEpiStoreF32><<<grid, 256, 0, st>>>(a, seg); break;
-    case kEpiSwigluFp8: gemm_fp8_plain_kernel<kEpiSwigluFp8><<<grid, 256, 0, st>>>(a, seg); break;
-    default: return 2;
+    case kEpiStore: rc = launch_pair<kEpiStore>(a, seg, st, err); break;
+    case kEpiResid: rc = launch_pair<kEpiResid>(a, seg, st, err); break;
+    case kEpiSwiglu: rc = launch_pair<kEpiSwiglu>(a, seg, st, err); break;
+    case kEpiStoreF32: rc = launch_pair<kEpiStoreF32>(a, seg, st, err); break;
+    default: rc = launch_pair<kEpiSwigluFp8>(a, seg, st, err); break;
   }
-  if (cudaGetLastError() == cudaSuccess) return 0;
-  *err = "gemm_fp8: kernel launch failed";
-  return 2;
+  if (rc && err->empty()) *err = "gemm_fp8: kernel launch failed";
+  return rc;
 }
 
 }  // namespace u15

@@ -227,6 +227,11 @@ bool attention_tc_serves(int mode, int tk, const int32_t* t_index);
 int make_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols,
                 uint32_t box_rows, int elsize, std::string* err);
 
+// A TMA map over packed fp8 scales (u15_fp8.cuh): [rowblks][groups] tiles of
+// 512 bytes, box of one group x box_rowblks tiles, zero fill.
+int make_tma_fp8_scales(CUtensorMap* out, const void* ptr, uint64_t rowblks, uint64_t groups,
+                        uint32_t box_rowblks, std::string* err);
+
 // Sage prologue: K smoothing (mean over tk keys per kv head and channel),
 // int8 quantisation of Q per 64-row block and of the smoothed K per 32-key
 // block (the reference's bq = 64, bk = 32).
