@@ -212,10 +212,14 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           const int nk = min(kKps, p.n_kblk - kb);
           const uint32_t fb = mapa_shared(full0 + 8 * s, 0);
           const uint32_t st = smem_u32(smem) + s * kStageBytes;
-          mbar_arrive_expect_tx_cluster(fb, nk * tx + tx_sf);
-          const uint32_t sf = st + 2 * kKps * kTileBytes;
-          tma_load_sf_pair(sf, &tmSA, kb >> 2, arow >> 7, fb);
-          tma_load_sf_pair(sf + kFp8SfTile, half ? &tmSBh : &tmSB, kb >> 2, sblk, fb);
+          // a scale tile serves four k-blocks: it comes with the first of them
+          const bool sfs = (kb & 3) == 0;
+          mbar_arrive_expect_tx_cluster(fb, nk * tx + (sfs ? tx_sf : 0));
+          if (sfs) {
+            const uint32_t sf = st + 2 * kKps * kTileBytes;
+            tma_load_sf_pair(sf, &tmSA, kb >> 2, arow >> 7, fb);
+            tma_load_sf_pair(sf + kFp8SfTile, half ? &tmSBh : &tmSB, kb >> 2, sblk, fb);
+          }
           for (int hk = 0; hk < nk; ++hk) {
             const int kx = (kb + hk) * 128;
             tma_load_2d_pair(st + hk * kTileBytes, &tmA, kx, arow, fb);
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
     // ---------------- MMA issuer (leader only) ----------------
     if (lane_id() == 0) {
       if (leader) {
-        uint32_t it = 0;
+        uint32_t it = 0, sf_set = 0;
         int lt = 0;
         bool ok = true;
         for (int t = pair; t < n_tiles && ok; t += n_pairs, ++lt) {
@@ -258,11 +262,13 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
             tc_fence_after();
             const int nk = min(kKps, p.n_kblk - kb);
             const uint32_t st = smem_u32(smem) + s * kStageBytes;
-            const uint32_t sf = st + 2 * kKps * kTileBytes;
-            const uint32_t sfa = tmem_base + kSfCol + (it & 1) * 16, sfb = sfa + 4;
-            sf_copy_pair(sfa, smem_desc_sf(sf));
-            sf_copy_pair(sfb, smem_desc_sf(sf + kFp8SfTile));
-            if (!half) sf_copy_pair(sfb + 4, smem_desc_sf(sf + 2 * kFp8SfTile));
+            const uint32_t sfa = tmem_base + kSfCol + sf_set * 16, sfb = sfa + 4;
+            if ((kb & 3) == 0) {
+              const uint32_t sf = st + 2 * kKps * kTileBytes;
+              sf_copy_pair(sfa, smem_desc_sf(sf));
+              sf_copy_pair(sfb, smem_desc_sf(sf + kFp8SfTile));
+              if (!half) sf_copy_pair(sfb + 4, smem_desc_sf(sf + 2 * kFp8SfTile));
+            }
             for (int hk = 0; hk < nk; ++hk) {
               const uint32_t a0 = st + hk * kTileBytes, b0 = st + (kKps + hk) * kTileBytes;
               const uint32_t id = idesc | idesc_scale_byte((kb + hk) & 3);
@@ -272,7 +278,9 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
                               sfa, sfb, ((kb + hk) | k) != 0);
             }
             mma_commit_pair_mc(empty0 + 8 * s, 0x3);
+            if ((kb & 3) + kKps >= 4) sf_set ^= 1;
           }
+          sf_set ^= (p.n_kblk & 3) != 0;   // a tile that ended inside a group
           if (!ok) break;
           mma_commit_pair_mc(accf0 + 8 * (lt & 1), 0x3);
         }
