@@ -413,6 +413,283 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
   }
 }
 
+// ---------------------------------------------------------------------
+// Few rows: the weights are the bytes that count. A tile is 128 weight rows
+// (SwiGLU: the 128 gate rows and the 128 up rows that go with them) by MT
+// activation rows, the weights as the MMA's M = 128 side, so a lane of the
+// accumulator is an output column and its columns are the activation rows.
+// The k-blocks of a tile are split over the CTAs of a cluster; their partial
+// sums meet in shared memory, each CTA adding (in rank order) and finishing
+// its share of the rows. Two CTAs fit an SM, which keeps ~200 KB of weights
+// in flight there.
+//   warp 0     TMA producer, one k-block a stage
+//   warp 1     MMA issuer
+//   warps 2-5  TMEM -> shared memory, the sum over the cluster, the epilogue
+// ---------------------------------------------------------------------
+constexpr int kThreadsFew = 192;
+constexpr int kFewRows = 128;       // rows up to which this form runs
+constexpr int kFewPrefetch = 16;    // k-blocks a CTA sends towards L2 ahead of its loads
+
+template <int MT, bool GU>
+struct FewCfg {
+  static constexpr int kA = GU ? 2 * kTileBytes : kTileBytes;
+  static constexpr int kB = MT * 128;
+  static constexpr int kStage = kA + kB + 2048;            // + the scale tiles
+  static constexpr int kPerSm = GU && MT == 128 ? 1 : 2;   // 512 TMEM columns: alone on its SM
+  static constexpr int kStages = (kPerSm == 1 ? 4 : (114000 - 2048) / kStage);
+  static constexpr int kSmem = kStages * kStage + 1024 /*align*/ + 1024 /*bars, amax*/;
+  static constexpr int kAcc = GU ? 2 * MT : MT;            // accumulator columns
+  static constexpr int kSf = GU ? 12 : 8;                  // scale columns of a set, two sets
+  static constexpr int kCols = kAcc + 2 * kSf <= 32    ? 32
+                               : kAcc + 2 * kSf <= 64  ? 64
+                               : kAcc + 2 * kSf <= 128 ? 128
+                               : kAcc + 2 * kSf <= 256 ? 256
+                                                       : 512;
+  static_assert(kStages >= 2 && kStages * kStage >= kAcc * 512, "the partial sums take the ring");
+  // two CTAs an SM share its 512 TMEM columns, and a third never fits beside
+  // them (its allocation would wait for theirs while their clusters wait for it)
+  static_assert(kPerSm == 1 ? kSmem > 116736 : kCols <= 256 && kSmem > 77824 && kSmem <= 115712, "");
+};
+
+struct FewParams {
+  int M, N, n_kblk;
+  int nseg;
+  int seg_off[kMaxSeg + 1];
+  int seg_expert[kMaxSeg];
+  int unit_start[kMaxSeg + 1];
+  int sf_blk_expert;
+  void* y;
+  const bf16* resid;
+  const bf16* bias;
+  uint8_t* sy;
+  unsigned* err;
+};
+
+template <int MT, int EPI>
+__global__ void __launch_bounds__(kThreadsFew, 2)
+    gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmX,
+                        const __grid_constant__ CUtensorMap tmW,
+                        const __grid_constant__ CUtensorMap tmSX,
+                        const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ FewParams p)
+{
+  constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
+  using C = FewCfg<MT, GU>;
+  constexpr int NA = GU ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 3);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::kStages,
+                 accf = empty0 + 8 * C::kStages, drain = accf + 8, amaxb = drain + 8;
+
+  const uint32_t w = warp_id();
+  const int split = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster is the x axis
+  const int tile = blockIdx.y;
+  // the unit: an MT-row block of one segment
+  int s_ = 0;
+#pragma unroll 1
+  for (int k = 1; k < p.nseg; ++k)
+    if ((int)blockIdx.z >= p.unit_start[k]) s_ = k;
+  const int m0 = (p.seg_off[s_] / MT + ((int)blockIdx.z - p.unit_start[s_])) * MT;
+  const int lo = max(m0, p.seg_off[s_]) - m0, hi = min(m0 + MT, p.seg_off[s_ + 1]) - m0;
+  const int expert = p.seg_expert[s_];
+  const int kb0 = (int)((long)rank * p.n_kblk / split), kb1 = (int)((long)(rank + 1) * p.n_kblk / split);
+  const int wrow = expert * p.N + tile * 128 * NA;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    mbar_init(accf, 1);
+    mbar_init(drain, 1);
+    mbar_init(amaxb, 128);
+    fence_barrier_init();
+  }
+  if (w == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::kCols);
+    tmem_relinquish();
+  }
+  if (w == 0 && lane_id() == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmSW);
+    tma_prefetch_desc(&tmSX);
+    // the weights' first tiles start towards L2 while the previous kernel
+    // still runs (a prefetch reads nothing into this CTA: were they being
+    // written, L2 holds the new bytes when the loads come)
+    const int pf = min(kb1, kb0 + kFewPrefetch);
+    for (int kb = kb0; kb < pf; ++kb)
+      for (int h = 0; h < NA; ++h) tma_prefetch_2d(&tmW, kb * 128, wrow + 128 * h);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch();
+  griddep_wait();
+
+  if (w == 0) {
+    if (lane_id() == 0) {
+      int it = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % C::kStages, ph = (it / C::kStages) & 1;
+        if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) break;
+        const uint32_t st = smem_u32(smem) + s * C::kStage, fb = full0 + 8 * s;
+        const bool sfs = kb == kb0 || (kb & 3) == 0;   // a scale tile serves its four k-blocks
+        mbar_arrive_expect_tx(fb, C::kA + C::kB + (sfs ? (NA + 1) * kFp8SfTile : 0));
+        for (int h = 0; h < NA; ++h)
+          tma_load_2d(st + h * kTileBytes, &tmW, kb * 128, wrow + 128 * h, fb);
+        tma_load_2d(st + C::kA, &tmX, kb * 128, m0, fb);
+        if (sfs) {
+          const uint32_t sf = st + C::kA + C::kB;
+          tma_load_sf(sf, &tmSX, kb >> 2, m0 >> 7, fb);
+          for (int h = 0; h < NA; ++h)
+            tma_load_sf(sf + (1 + h) * kFp8SfTile, &tmSW, kb >> 2,
+                        expert * p.sf_blk_expert + tile * NA + h, fb);
+        }
+      }
+      for (int s = 0; s < C::kStages; ++s)   // every fill has landed before the CTA may exit
+        if (it > s) mbar_wait(full0 + 8 * s, ((it - 1 - s) / C::kStages) & 1, p.err, kDevWaitDrain);
+    }
+  } else if (w == 1) {
+    if (lane_id() == 0) {
+      const uint32_t idesc = idesc_e4m3(128, MT);
+      int it = 0;
+      uint32_t set = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % C::kStages, ph = (it / C::kStages) & 1;
+        if (!mbar_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t st = smem_u32(smem) + s * C::kStage;
+        if (it != 0 && (kb & 3) == 0) set ^= 1;
+        const uint32_t sfx = tmem + C::kAcc + set * C::kSf, sfw = sfx + 4;
+        if (it == 0 || (kb & 3) == 0) {
+          const uint32_t sf = st + C::kA + C::kB;
+          sf_copy(sfx, smem_desc_sf(sf));
+          for (int h = 0; h < NA; ++h)
+            sf_copy(sfw + 4 * h, smem_desc_sf(sf + (1 + h) * kFp8SfTile));
+        }
+        const uint32_t id = idesc | idesc_scale_byte(kb & 3);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int h = 0; h < NA; ++h)
+            mma_e4m3(tmem + h * MT, smem_desc_sw128(st + h * kTileBytes + k * 32),
+                     smem_desc_sw128(st + C::kA + k * 32), id, sfw + 4 * h, sfx, (it | k) != 0);
+        mma_commit(empty0 + 8 * s);
+      }
+      if (ok) mma_commit(accf);
+      mma_commit(drain);
+      mbar_wait(drain, 0, p.err, kDevWaitDrain);
+    }
+  }
+
+  float* part = reinterpret_cast<float*>(smem);   // [NA][MT rows][128 columns], over the ring
+  const int wq = (int)(w & 3), n = wq * 32 + (int)lane_id();
+  bool ok = true;
+  if (w >= 2) {
+    // every MMA of this CTA has completed, and with them every load
+    ok = mbar_wait(accf, 0, p.err, kDevWaitAccFull);
+    tc_fence_after();
+    const uint32_t tb = tmem + ((uint32_t)(wq * 32) << 16);
+#pragma unroll 1
+    for (int c = (lo & ~15); c < hi; c += 16) {
+#pragma unroll
+      for (int h = 0; h < NA; ++h) {
+        uint32_t r[16];
+        tmem_ld16(tb + h * MT + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(h * MT + c + i) * 128 + n] = __uint_as_float(r[i]);
+      }
+    }
+  }
+  __syncthreads();
+  cluster_sync();   // every CTA's partial sums are in its shared memory
+
+  if (w >= 2 && ok) {
+    const uint32_t own = smem_u32(part);
+    float* am = reinterpret_cast<float*>(smem + C::kStages * C::kStage + 512);   // [2][4 rows][4 warps]
+    (void)am;
+    uint32_t peer[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) peer[q] = q < split ? mapa_shared(own, q) : 0;
+    auto total = [&](int at) {
+      float v[8], t = 0.0f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = q < split ? ld_cluster(peer[q] + at * 4) : 0.0f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) t += v[q];
+      return t;
+    };
+    // four rows a step, so that their loads are in flight together
+    constexpr int R = 4;
+    const int ncols = GU ? p.N / 2 : p.N, col = tile * 128 + n;
+    uint32_t ph = 0;
+    for (int j0 = lo + rank; j0 < hi; j0 += R * split) {
+      float v[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int j = min(j0 + i * split, hi - 1);
+        v[i] = total(j * 128 + n);
+        if constexpr (GU) v[i] = swiglu1(v[i], total((MT + j) * 128 + n));
+      }
+      if constexpr (EPI == kEpiSwigluFp8) {
+        // a row's largest of 128 outputs, over the four warps
+        float* mine = am + (ph & 1) * (4 * R);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float m = fabsf(v[i]);
+          const uint32_t u = __reduce_max_sync(0xffffffffu, m == m ? __float_as_uint(m) : 0u);
+          if (lane_id() == 0) mine[i * 4 + wq] = __uint_as_float(u);
+        }
+        mbar_arrive(amaxb);
+        if (!mbar_wait(amaxb, ph & 1, p.err, kDevWaitAccFull)) break;
+        ++ph;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (j0 + i * split >= hi) break;
+          const long row = m0 + j0 + i * split;
+          const uint32_t sb = fp8_scale_byte(fmaxf(fmaxf(mine[i * 4], mine[i * 4 + 1]),
+                                                   fmaxf(mine[i * 4 + 2], mine[i * 4 + 3])));
+          const float q = __fmaf_rn(v[i], 0.0f, v[i] * fp8_inv_scale(sb));
+          static_cast<uint8_t*>(p.y)[row * ncols + col] =
+              (uint8_t)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+          if (n == 0) p.sy[fp8_scale_at(row, tile, fp8_groups(ncols))] = (uint8_t)sb;
+        }
+      } else {
+        if (col >= ncols) continue;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (j0 + i * split >= hi) break;
+          const long at = (long)(m0 + j0 + i * split) * ncols + col;
+          float t = v[i];
+          if (p.bias != nullptr) t += bf2f(p.bias[(long)expert * p.N + col]);
+          if constexpr (EPI == kEpiResid) t += bf2f(p.resid[at]);
+          if constexpr (EPI == kEpiStoreF32)
+            static_cast<float*>(p.y)[at] = t;
+          else
+            static_cast<bf16*>(p.y)[at] = f2bf(t);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the peers have read this CTA's partial sums
+  if (w == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+}
+
 // Persistent grid: as many pairs as can be resident at once (not every SM has
 // a usable partner).
 template <int EPI>
@@ -490,6 +767,89 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
   return cudaLaunchKernelEx(&cfg, k, ma, mb, mbh, msa, msb, msbh, p) == cudaSuccess ? 0 : 2;
 }
 
+// How many CTAs share a tile's k-blocks: the cluster size with the least time
+// in units of one k-block, rounds of the grid (two CTAs an SM) times the k-blocks of a CTA
+// plus what the exchange of the partial sums costs.
+inline int few_split(long tiles, int n_kblk, int slots)
+{
+  int best = 1;
+  long best_cost = -1;
+  for (int s = 1; s <= 8 && s <= n_kblk; ++s) {
+    const long rounds = (tiles * s + slots - 1) / slots;
+    const long cost = rounds * ((n_kblk + s - 1) / s + 4) + (s > 1 ? s : 0);
+    if (best_cost < 0 || cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+template <int MT, int EPI>
+int launch_few(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+{
+  static std::atomic<uint64_t> attr_set;
+  constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
+  using C = FewCfg<MT, GU>;
+  FewParams p{};
+  p.M = a.M;
+  p.N = a.N;
+  p.n_kblk = fp8_blocks(a.K);
+  p.sf_blk_expert = (a.N + 127) / 128;
+  p.y = a.y;
+  p.resid = static_cast<const bf16*>(a.resid);
+  p.bias = static_cast<const bf16*>(a.bias);
+  p.sy = a.sy;
+  p.err = a.dev_err;
+  p.nseg = seg.nseg;
+  int units = 0;
+  for (int s = 0; s < seg.nseg; ++s) {
+    p.seg_off[s] = seg.off[s];
+    p.seg_expert[s] = seg.expert[s];
+    p.unit_start[s] = units;
+    if (seg.off[s + 1] > seg.off[s]) units += (seg.off[s + 1] + MT - 1) / MT - seg.off[s] / MT;
+  }
+  p.seg_off[seg.nseg] = seg.off[seg.nseg];
+  p.unit_start[seg.nseg] = units;
+  const int tiles = GU ? a.N / 256 : (a.N + 127) / 128;
+  CUtensorMap mx, mw, msx, msw;
+  const uint64_t groups = fp8_groups(a.K);
+  if (make_tma_2d(&mx, a.xq, a.M, a.K, MT, 1, err) ||
+      make_tma_2d(&mw, a.wq, (uint64_t)a.N * a.n_experts, a.K, 128, 1, err) ||
+      make_tma_fp8_scales(&msx, a.sx, (a.M + 127) / 128, groups, 1, err) ||
+      make_tma_fp8_scales(&msw, a.sw, (uint64_t)p.sf_blk_expert * a.n_experts, groups, 1, err))
+    return 2;
+  auto k = gemm_fp8_few_kernel<MT, EPI>;
+  if (!smem_attr_once(k, C::kSmem, attr_set)) return 2;
+  const int split = few_split((long)tiles * units, p.n_kblk, C::kPerSm * a.num_sms);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(split, tiles, units);
+  cfg.blockDim = dim3(kThreadsFew);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attrs[2] = {};
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = split;
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, mx, mw, msx, msw, p) == cudaSuccess ? 0 : 2;
+}
+
+template <int EPI>
+int launch_rows(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+{
+  const int tiles = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8 ? a.N / 256 : (a.N + 127) / 128;
+  if (a.M > kFewRows || tiles > 65535) return launch_pair<EPI>(a, seg, st, err);
+  if (a.M <= 16) return launch_few<16, EPI>(a, seg, st, err);
+  if (a.M <= 32) return launch_few<32, EPI>(a, seg, st, err);
+  if (a.M <= 64) return launch_few<64, EPI>(a, seg, st, err);
+  return launch_few<128, EPI>(a, seg, st, err);
+}
+
 }  // namespace
 
 int gemm_fp8(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
@@ -497,11 +857,11 @@ int gemm_fp8(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::str
   err->clear();
   int rc;
   switch (a.epilogue) {
-    case kEpiStore: rc = launch_pair<kEpiStore>(a, seg, st, err); break;
-    case kEpiResid: rc = launch_pair<kEpiResid>(a, seg, st, err); break;
-    case kEpiSwiglu: rc = launch_pair<kEpiSwiglu>(a, seg, st, err); break;
-    case kEpiStoreF32: rc = launch_pair<kEpiStoreF32>(a, seg, st, err); break;
-    default: rc = launch_pair<kEpiSwigluFp8>(a, seg, st, err); break;
+    case kEpiStore: rc = launch_rows<kEpiStore>(a, seg, st, err); break;
+    case kEpiResid: rc = launch_rows<kEpiResid>(a, seg, st, err); break;
+    case kEpiSwiglu: rc = launch_rows<kEpiSwiglu>(a, seg, st, err); break;
+    case kEpiStoreF32: rc = launch_rows<kEpiStoreF32>(a, seg, st, err); break;
+    default: rc = launch_rows<kEpiSwigluFp8>(a, seg, st, err); break;
   }
   if (rc && err->empty()) *err = "gemm_fp8: kernel launch failed";
   return rc;
