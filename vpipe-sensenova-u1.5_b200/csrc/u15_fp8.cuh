@@ -69,6 +69,20 @@ __device__ __forceinline__ uint2 fp8_codes8(const float (&v)[8], float inv)
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
+// the same for four values
+__device__ __forceinline__ uint32_t fp8_codes4(const float (&v)[4], float inv)
+{
+  uint32_t h[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float2 f;
+    f.x = __fmaf_rn(v[2 * i], 0.0f, v[2 * i] * inv);
+    f.y = __fmaf_rn(v[2 * i + 1], 0.0f, v[2 * i + 1] * inv);
+    h[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  }
+  return h[0] | (h[1] << 16);
+}
+
 // two e4m3 values as floats (exact)
 __device__ __forceinline__ float2 fp8_pair(uint32_t lo16)
 {
@@ -93,6 +107,39 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N)
 }
 // the byte of the scale words to use, for B at bit 4 and for A at bit 29
 __device__ __forceinline__ uint32_t idesc_scale_byte(uint32_t id) { return (id << 4) | (id << 29); }
+
+// One lane of a converged warp. The producers and issuers here run their
+// loops with the whole warp and let this lane issue: addresses and
+// descriptors then stay in uniform registers, which a loop inside
+// `if (lane == 0)` has to move there for every instruction (an issuer of four
+// MMAs a stage took ~105 cycles an MMA that way).
+__device__ __forceinline__ bool elect_one()
+{
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// The bounded waits for a whole warp: every lane gets the same answer, so the
+// warp stays converged where a wait runs out.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, unsigned* err, unsigned code)
+{
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+__device__ __forceinline__ bool warp_wait_probe(uint32_t bar, uint32_t parity, unsigned* err,
+                                                unsigned code)
+{
+  return __all_sync(0xffffffffu, mbar_wait_probe(bar, parity, err, code));
+}
+__device__ __forceinline__ bool warp_wait_cluster_probe(uint32_t bar, uint32_t parity, unsigned* err,
+                                                        unsigned code)
+{
+  return __all_sync(0xffffffffu, mbar_wait_cluster_probe(bar, parity, err, code));
+}
 
 // a packed 512-byte tile in shared memory as 32 rows of 16 bytes: no swizzle,
 // 8-row groups 128 bytes apart
@@ -179,11 +226,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
         "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-// a float of another CTA of the cluster's shared memory
-__device__ __forceinline__ float ld_cluster(uint32_t addr)
+// 16 bytes of another CTA of the cluster's shared memory
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr)
 {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 

@@ -9,6 +9,7 @@
 #include "u15_kernels.h"
 
 #include <algorithm>
+#include <mutex>
 
 namespace u15 {
 
@@ -189,106 +190,117 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 
   const int n_tiles = p.n_full + 2 * (p.n_units * p.n_nblk - p.n_full);
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const uint32_t base = smem_u32(smem);
 
   if (w == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
-    if (lane_id() == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = pair; t < n_tiles && ok; t += n_pairs) {
-        const PairTile ti = pair_tile(p, t);
-        const bool half = ti.half >= 0;
-        const int arow = ti.m0 + 128 * (int)rank;
-        const int brow = ti.expert * p.N + ti.nb * 256 + (half ? 128 * ti.half + 64 * (int)rank : 128 * (int)rank);
-        const int sblk = ti.expert * p.sf_blk_expert + ti.nb * 2 + (half ? ti.half : 0);
-        const uint32_t tx = kTileBytes + (half ? kTileBytes / 2 : kTileBytes);
-        const uint32_t tx_sf = half ? 2 * kFp8SfTile : 3 * kFp8SfTile;
-        for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
-          const uint32_t s = it % kStg, ph = (it / kStg) & 1;
-          if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) {
-            ok = false;
-            break;
-          }
-          const int nk = min(kKps, p.n_kblk - kb);
-          const uint32_t fb = mapa_shared(full0 + 8 * s, 0);
-          const uint32_t st = smem_u32(smem) + s * kStageBytes;
-          // a scale tile serves four k-blocks: it comes with the first of them
-          const bool sfs = (kb & 3) == 0;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = pair; t < n_tiles && ok; t += n_pairs) {
+      const PairTile ti = pair_tile(p, t);
+      const bool half = ti.half >= 0;
+      const int arow = ti.m0 + 128 * (int)rank;
+      const int brow = ti.expert * p.N + ti.nb * 256 +
+                       (half ? 128 * ti.half + 64 * (int)rank : 128 * (int)rank);
+      const int sblk = ti.expert * p.sf_blk_expert + ti.nb * 2 + (half ? ti.half : 0);
+      const uint32_t tx = kTileBytes + (half ? kTileBytes / 2 : kTileBytes);
+      const uint32_t tx_sf = half ? 2 * kFp8SfTile : 3 * kFp8SfTile;
+      const CUtensorMap *mb = half ? &tmBh : &tmB, *msb = half ? &tmSBh : &tmSB;
+      for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
+        const uint32_t s = it % kStg, ph = (it / kStg) & 1;
+        if (!warp_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) {
+          ok = false;
+          break;
+        }
+        const int nk = min(kKps, p.n_kblk - kb);
+        const uint32_t fb = mapa_shared(full0 + 8 * s, 0);
+        const uint32_t st = base + s * kStageBytes;
+        // a scale tile serves four k-blocks: it comes with the first of them
+        const bool sfs = (kb & 3) == 0;
+        if (elect_one()) {
           mbar_arrive_expect_tx_cluster(fb, nk * tx + (sfs ? tx_sf : 0));
           if (sfs) {
             const uint32_t sf = st + 2 * kKps * kTileBytes;
             tma_load_sf_pair(sf, &tmSA, kb >> 2, arow >> 7, fb);
-            tma_load_sf_pair(sf + kFp8SfTile, half ? &tmSBh : &tmSB, kb >> 2, sblk, fb);
+            tma_load_sf_pair(sf + kFp8SfTile, msb, kb >> 2, sblk, fb);
           }
-          for (int hk = 0; hk < nk; ++hk) {
+#pragma unroll
+          for (int hk = 0; hk < kKps; ++hk) {
+            if (hk >= nk) break;
             const int kx = (kb + hk) * 128;
             tma_load_2d_pair(st + hk * kTileBytes, &tmA, kx, arow, fb);
-            tma_load_2d_pair(st + (kKps + hk) * kTileBytes, half ? &tmBh : &tmB, kx, brow, fb);
+            tma_load_2d_pair(st + (kKps + hk) * kTileBytes, mb, kx, brow, fb);
           }
         }
+        __syncwarp();
       }
-      // unwinding (leader): the last fill of every stage, both CTAs' halves,
-      // has landed once the leader's full barrier for it completes
-      if (leader) {
-        for (uint32_t s = 0; s < kStg; ++s) {
-          if (it > s) {
-            const uint32_t last = ((it - 1 - s) / kStg) * kStg + s;
-            mbar_wait(full0 + 8 * s, (last / kStg) & 1, p.err, kDevWaitDrain);
-          }
+    }
+    // unwinding (leader): the last fill of every stage, both CTAs' halves,
+    // has landed once the leader's full barrier for it completes
+    if (leader) {
+      for (uint32_t s = 0; s < kStg; ++s) {
+        if (it > s) {
+          const uint32_t last = ((it - 1 - s) / kStg) * kStg + s;
+          warp_wait(full0 + 8 * s, (last / kStg) & 1, p.err, kDevWaitDrain);
         }
       }
     }
   } else if (w == 1) {
     // ---------------- MMA issuer (leader only) ----------------
-    if (lane_id() == 0) {
-      if (leader) {
-        uint32_t it = 0, sf_set = 0;
-        int lt = 0;
-        bool ok = true;
-        for (int t = pair; t < n_tiles && ok; t += n_pairs, ++lt) {
-          const bool half = t >= p.n_full;
-          const uint32_t idesc = half ? idesc_e4m3(256, 128) : idesc_e4m3(256, 256);
-          // the previous tile's shared columns have been read (and with them
-          // all of the tile before it)
-          if (lt > 0 && !mbar_wait_cluster_probe(accr, (lt - 1) & 1, p.err, kDevWaitAccEmpty)) break;
+    if (leader) {
+      uint32_t it = 0, sf_set = 0;
+      int lt = 0;
+      bool ok = true;
+      for (int t = pair; t < n_tiles && ok; t += n_pairs, ++lt) {
+        const bool half = t >= p.n_full;
+        const uint32_t idesc = half ? idesc_e4m3(256, 128) : idesc_e4m3(256, 256);
+        // the previous tile's shared columns have been read (and with them
+        // all of the tile before it)
+        if (lt > 0 && !warp_wait_cluster_probe(accr, (lt - 1) & 1, p.err, kDevWaitAccEmpty)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (lt & 1) * kAccStep;
+        for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
+          const uint32_t s = it % kStg, ph = (it / kStg) & 1;
+          if (!warp_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
+            ok = false;
+            break;
+          }
           tc_fence_after();
-          const uint32_t d_tmem = tmem_base + (lt & 1) * kAccStep;
-          for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
-            const uint32_t s = it % kStg, ph = (it / kStg) & 1;
-            if (!mbar_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const int nk = min(kKps, p.n_kblk - kb);
-            const uint32_t st = smem_u32(smem) + s * kStageBytes;
-            const uint32_t sfa = tmem_base + kSfCol + sf_set * 16, sfb = sfa + 4;
+          const int nk = min(kKps, p.n_kblk - kb);
+          const uint32_t st = base + s * kStageBytes;
+          if ((kb & 3) == 0) sf_set ^= 1;
+          const uint32_t sfa = tmem_base + kSfCol + sf_set * 16, sfb = sfa + 4;
+          const uint64_t ad = smem_desc_sw128(st), bd = smem_desc_sw128(st + kKps * kTileBytes);
+          if (elect_one()) {
             if ((kb & 3) == 0) {
-              const uint32_t sf = st + 2 * kKps * kTileBytes;
-              sf_copy_pair(sfa, smem_desc_sf(sf));
-              sf_copy_pair(sfb, smem_desc_sf(sf + kFp8SfTile));
-              if (!half) sf_copy_pair(sfb + 4, smem_desc_sf(sf + 2 * kFp8SfTile));
+              const uint64_t sf = smem_desc_sf(st + 2 * kKps * kTileBytes);
+              sf_copy_pair(sfa, sf);
+              sf_copy_pair(sfb, sf + (kFp8SfTile >> 4));
+              if (!half) sf_copy_pair(sfb + 4, sf + 2 * (kFp8SfTile >> 4));
             }
-            for (int hk = 0; hk < nk; ++hk) {
-              const uint32_t a0 = st + hk * kTileBytes, b0 = st + (kKps + hk) * kTileBytes;
+#pragma unroll
+            for (int hk = 0; hk < kKps; ++hk) {
+              if (hk >= nk) break;
               const uint32_t id = idesc | idesc_scale_byte((kb + hk) & 3);
+              // K = 32 steps are 32 bytes, 2 descriptor units, apart
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                mma_e4m3_pair(d_tmem, smem_desc_sw128(a0 + k * 32), smem_desc_sw128(b0 + k * 32), id,
-                              sfa, sfb, ((kb + hk) | k) != 0);
+                mma_e4m3_pair(d_tmem, ad + hk * (kTileBytes >> 4) + k * 2,
+                              bd + hk * (kTileBytes >> 4) + k * 2, id, sfa, sfb,
+                              ((kb + hk) | k) != 0);
             }
             mma_commit_pair_mc(empty0 + 8 * s, 0x3);
-            if ((kb & 3) + kKps >= 4) sf_set ^= 1;
           }
-          sf_set ^= (p.n_kblk & 3) != 0;   // a tile that ended inside a group
-          if (!ok) break;
-          mma_commit_pair_mc(accf0 + 8 * (lt & 1), 0x3);
+          __syncwarp();
         }
-        mma_commit_pair_mc(drain, 0x3);
+        if (ok && elect_one()) mma_commit_pair_mc(accf0 + 8 * (lt & 1), 0x3);
+        __syncwarp();
       }
-      // both CTAs: every MMA that writes this CTA's TMEM has completed
-      mbar_wait(drain, 0, p.err, kDevWaitDrain);
+      if (elect_one()) mma_commit_pair_mc(drain, 0x3);
+      __syncwarp();
     }
+    // both CTAs: every MMA that writes this CTA's TMEM has completed
+    warp_wait(drain, 0, p.err, kDevWaitDrain);
   } else {
     // ---------------- epilogue (warps 2..9, both CTAs) ----------------
     const int wq = (int)(w & 3), wh = (int)(w - 2) >> 2;   // lane quadrant, half of the columns
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
       const PairTile ti = pair_tile(p, t);
       const bool half = ti.half >= 0;
       const int acc = lt & 1;
-      if (!mbar_wait(accf0 + 8 * acc, (lt >> 1) & 1, p.err, kDevWaitAccFull)) break;
+      if (!warp_wait(accf0 + 8 * acc, (lt >> 1) & 1, p.err, kDevWaitAccFull)) break;
       tc_fence_after();
       const int row = ti.m0 + 128 * (int)rank + r_in;
       const bool row_ok = row >= ti.row_lo && row < ti.row_hi;
@@ -350,7 +362,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           float* am = amax_sm + acc * 256;
           am[wh * 128 + r_in] = m;
           mbar_arrive(amax0 + 8 * wq);
-          if (!mbar_wait(amax0 + 8 * wq, lt & 1, p.err, kDevWaitAccFull)) break;
+          if (!warp_wait(amax0 + 8 * wq, lt & 1, p.err, kDevWaitAccFull)) break;
           m = fmaxf(m, am[(wh ^ 1) * 128 + r_in]);
           const uint32_t sb = fp8_scale_byte(m);
           const float inv = fp8_inv_scale(sb);
@@ -424,11 +436,14 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 // in flight there.
 //   warp 0     TMA producer, one k-block a stage
 //   warp 1     MMA issuer
-//   warps 2-5  TMEM -> shared memory, the sum over the cluster, the epilogue
+//   warps 2-5  TMEM -> shared memory; then every warp: the sum over the
+//              cluster and the epilogue, a row a warp
 // ---------------------------------------------------------------------
 constexpr int kThreadsFew = 192;
 constexpr int kFewRows = 128;       // rows up to which this form runs
-constexpr int kFewPrefetch = 16;    // k-blocks a CTA sends towards L2 ahead of its loads
+constexpr int kFewPrefetch = 4;     // k-blocks a CTA sends towards L2 ahead of its loads
+constexpr int kMaxSplit = 8;        // the portable cluster size
+constexpr int kFewSetUp = 4;        // a CTA's set-up, in k-blocks
 
 template <int MT, bool GU>
 struct FewCfg {
@@ -437,7 +452,7 @@ struct FewCfg {
   static constexpr int kStage = kA + kB + 2048;            // + the scale tiles
   static constexpr int kPerSm = GU && MT == 128 ? 1 : 2;   // 512 TMEM columns: alone on its SM
   static constexpr int kStages = (kPerSm == 1 ? 4 : (114000 - 2048) / kStage);
-  static constexpr int kSmem = kStages * kStage + 1024 /*align*/ + 1024 /*bars, amax*/;
+  static constexpr int kSmem = kStages * kStage + 1024 /*align*/ + 256 /*bars*/;
   static constexpr int kAcc = GU ? 2 * MT : MT;            // accumulator columns
   static constexpr int kSf = GU ? 12 : 8;                  // scale columns of a set, two sets
   static constexpr int kCols = kAcc + 2 * kSf <= 32    ? 32
@@ -465,6 +480,41 @@ struct FewParams {
   unsigned* err;
 };
 
+// four columns of a row, of which the first n exist; `whole`: all four, and
+// rows are a multiple of four columns
+__device__ __forceinline__ void add4(float (&v)[4], const bf16* src, bool whole, int n)
+{
+  if (whole && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+    const uint2 u = *reinterpret_cast<const uint2*>(src);
+    const float2 a = unpack_bf2(u.x), b = unpack_bf2(u.y);
+    v[0] += a.x; v[1] += a.y; v[2] += b.x; v[3] += b.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) v[i] += bf2f(src[i]);
+  }
+}
+__device__ __forceinline__ void store4(bf16* dst, const float (&v)[4], bool whole, int n)
+{
+  if (whole && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) dst[i] = f2bf(v[i]);
+  }
+}
+__device__ __forceinline__ void store4(float* dst, const float (&v)[4], bool whole, int n)
+{
+  if (whole && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) dst[i] = v[i];
+  }
+}
+
 template <int MT, int EPI>
 __global__ void __launch_bounds__(kThreadsFew, 2)
     gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmX,
@@ -479,9 +529,9 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 3);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 2);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::kStages,
-                 accf = empty0 + 8 * C::kStages, drain = accf + 8, amaxb = drain + 8;
+                 accf = empty0 + 8 * C::kStages, drain = accf + 8;
 
   const uint32_t w = warp_id();
   const int split = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster is the x axis
@@ -496,6 +546,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
   const int expert = p.seg_expert[s_];
   const int kb0 = (int)((long)rank * p.n_kblk / split), kb1 = (int)((long)(rank + 1) * p.n_kblk / split);
   const int wrow = expert * p.N + tile * 128 * NA;
+  const uint32_t base = smem_u32(smem);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -504,7 +555,6 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
     }
     mbar_init(accf, 1);
     mbar_init(drain, 1);
-    mbar_init(amaxb, 128);
     fence_barrier_init();
   }
   if (w == 1) {
@@ -531,63 +581,72 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
   griddep_wait();
 
   if (w == 0) {
-    if (lane_id() == 0) {
-      int it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::kStages, ph = (it / C::kStages) & 1;
-        if (!mbar_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) break;
-        const uint32_t st = smem_u32(smem) + s * C::kStage, fb = full0 + 8 * s;
-        const bool sfs = kb == kb0 || (kb & 3) == 0;   // a scale tile serves its four k-blocks
+    int it = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      const int s = it % C::kStages, ph = (it / C::kStages) & 1;
+      if (!warp_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) break;
+      const uint32_t st = base + s * C::kStage, fb = full0 + 8 * s;
+      const bool sfs = kb == kb0 || (kb & 3) == 0;   // a scale tile serves its four k-blocks
+      if (elect_one()) {
         mbar_arrive_expect_tx(fb, C::kA + C::kB + (sfs ? (NA + 1) * kFp8SfTile : 0));
+#pragma unroll
         for (int h = 0; h < NA; ++h)
           tma_load_2d(st + h * kTileBytes, &tmW, kb * 128, wrow + 128 * h, fb);
         tma_load_2d(st + C::kA, &tmX, kb * 128, m0, fb);
         if (sfs) {
           const uint32_t sf = st + C::kA + C::kB;
           tma_load_sf(sf, &tmSX, kb >> 2, m0 >> 7, fb);
+#pragma unroll
           for (int h = 0; h < NA; ++h)
             tma_load_sf(sf + (1 + h) * kFp8SfTile, &tmSW, kb >> 2,
                         expert * p.sf_blk_expert + tile * NA + h, fb);
         }
       }
-      for (int s = 0; s < C::kStages; ++s)   // every fill has landed before the CTA may exit
-        if (it > s) mbar_wait(full0 + 8 * s, ((it - 1 - s) / C::kStages) & 1, p.err, kDevWaitDrain);
+      __syncwarp();
     }
+    for (int s = 0; s < C::kStages; ++s)   // every fill has landed before the CTA may exit
+      if (it > s) warp_wait(full0 + 8 * s, ((it - 1 - s) / C::kStages) & 1, p.err, kDevWaitDrain);
   } else if (w == 1) {
-    if (lane_id() == 0) {
-      const uint32_t idesc = idesc_e4m3(128, MT);
-      int it = 0;
-      uint32_t set = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::kStages, ph = (it / C::kStages) & 1;
-        if (!mbar_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t st = smem_u32(smem) + s * C::kStage;
-        if (it != 0 && (kb & 3) == 0) set ^= 1;
-        const uint32_t sfx = tmem + C::kAcc + set * C::kSf, sfw = sfx + 4;
+    constexpr uint32_t idesc = idesc_e4m3(128, MT);
+    int it = 0;
+    uint32_t set = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      const int s = it % C::kStages, ph = (it / C::kStages) & 1;
+      if (!warp_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t st = base + s * C::kStage;
+      if (it != 0 && (kb & 3) == 0) set ^= 1;
+      const uint32_t sfx = tmem + C::kAcc + set * C::kSf, sfw = sfx + 4;
+      const uint32_t id = idesc | idesc_scale_byte(kb & 3);
+      const uint64_t ad = smem_desc_sw128(st), bd = smem_desc_sw128(st + C::kA);
+      if (elect_one()) {
         if (it == 0 || (kb & 3) == 0) {
-          const uint32_t sf = st + C::kA + C::kB;
-          sf_copy(sfx, smem_desc_sf(sf));
-          for (int h = 0; h < NA; ++h)
-            sf_copy(sfw + 4 * h, smem_desc_sf(sf + (1 + h) * kFp8SfTile));
+          const uint64_t sf = smem_desc_sf(st + C::kA + C::kB);
+          sf_copy(sfx, sf);
+#pragma unroll
+          for (int h = 0; h < NA; ++h) sf_copy(sfw + 4 * h, sf + (1 + h) * (kFp8SfTile >> 4));
         }
-        const uint32_t id = idesc | idesc_scale_byte(kb & 3);
+        // K = 32 steps are 32 bytes, 2 descriptor units, apart
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int h = 0; h < NA; ++h)
-            mma_e4m3(tmem + h * MT, smem_desc_sw128(st + h * kTileBytes + k * 32),
-                     smem_desc_sw128(st + C::kA + k * 32), id, sfw + 4 * h, sfx, (it | k) != 0);
+            mma_e4m3(tmem + h * MT, ad + h * (kTileBytes >> 4) + k * 2, bd + k * 2, id, sfw + 4 * h,
+                     sfx, (it | k) != 0);
         mma_commit(empty0 + 8 * s);
       }
+      __syncwarp();
+    }
+    if (elect_one()) {
       if (ok) mma_commit(accf);
       mma_commit(drain);
-      mbar_wait(drain, 0, p.err, kDevWaitDrain);
     }
+    __syncwarp();
+    warp_wait(drain, 0, p.err, kDevWaitDrain);
   }
 
   float* part = reinterpret_cast<float*>(smem);   // [NA][MT rows][128 columns], over the ring
@@ -595,7 +654,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
   bool ok = true;
   if (w >= 2) {
     // every MMA of this CTA has completed, and with them every load
-    ok = mbar_wait(accf, 0, p.err, kDevWaitAccFull);
+    ok = warp_wait(accf, 0, p.err, kDevWaitAccFull);
     tc_fence_after();
     const uint32_t tb = tmem + ((uint32_t)(wq * 32) << 16);
 #pragma unroll 1
@@ -613,70 +672,52 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
   __syncthreads();
   cluster_sync();   // every CTA's partial sums are in its shared memory
 
-  if (w >= 2 && ok) {
-    const uint32_t own = smem_u32(part);
-    float* am = reinterpret_cast<float*>(smem + C::kStages * C::kStage + 512);   // [2][4 rows][4 warps]
-    (void)am;
-    uint32_t peer[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) peer[q] = q < split ? mapa_shared(own, q) : 0;
+  if (ok) {
+    // a warp finishes whole rows, four columns a lane: the sum over the
+    // cluster in rank order, and a row's largest needs no other warp
+    const uint32_t own = smem_u32(part) + lane_id() * 16;
+    const int ncols = GU ? p.N / 2 : p.N, col = tile * 128 + (int)lane_id() * 4;
     auto total = [&](int at) {
-      float v[8], t = 0.0f;
+      float4 v[8], t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = q < split ? ld_cluster(peer[q] + at * 4) : 0.0f;
+      for (int q = 0; q < 8; ++q)
+        v[q] = q < split ? ld_cluster4(mapa_shared(own, q) + at * 512) : t;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) t += v[q];
+      for (int q = 0; q < 8; ++q) {
+        t.x += v[q].x;
+        t.y += v[q].y;
+        t.z += v[q].z;
+        t.w += v[q].w;
+      }
       return t;
     };
-    // four rows a step, so that their loads are in flight together
-    constexpr int R = 4;
-    const int ncols = GU ? p.N / 2 : p.N, col = tile * 128 + n;
-    uint32_t ph = 0;
-    for (int j0 = lo + rank; j0 < hi; j0 += R * split) {
-      float v[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const int j = min(j0 + i * split, hi - 1);
-        v[i] = total(j * 128 + n);
-        if constexpr (GU) v[i] = swiglu1(v[i], total((MT + j) * 128 + n));
+    for (int j = lo + rank + (int)w * split; j < hi; j += (kThreadsFew / 32) * split) {
+      float4 t = total(j);
+      float v[4] = {t.x, t.y, t.z, t.w};
+      if constexpr (GU) {
+        t = total(MT + j);
+        v[0] = swiglu1(v[0], t.x);
+        v[1] = swiglu1(v[1], t.y);
+        v[2] = swiglu1(v[2], t.z);
+        v[3] = swiglu1(v[3], t.w);
       }
+      const long row = m0 + j;
       if constexpr (EPI == kEpiSwigluFp8) {
-        // a row's largest of 128 outputs, over the four warps
-        float* mine = am + (ph & 1) * (4 * R);
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const float m = fabsf(v[i]);
-          const uint32_t u = __reduce_max_sync(0xffffffffu, m == m ? __float_as_uint(m) : 0u);
-          if (lane_id() == 0) mine[i * 4 + wq] = __uint_as_float(u);
-        }
-        mbar_arrive(amaxb);
-        if (!mbar_wait(amaxb, ph & 1, p.err, kDevWaitAccFull)) break;
-        ++ph;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          if (j0 + i * split >= hi) break;
-          const long row = m0 + j0 + i * split;
-          const uint32_t sb = fp8_scale_byte(fmaxf(fmaxf(mine[i * 4], mine[i * 4 + 1]),
-                                                   fmaxf(mine[i * 4 + 2], mine[i * 4 + 3])));
-          const float q = __fmaf_rn(v[i], 0.0f, v[i] * fp8_inv_scale(sb));
-          static_cast<uint8_t*>(p.y)[row * ncols + col] =
-              (uint8_t)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-          if (n == 0) p.sy[fp8_scale_at(row, tile, fp8_groups(ncols))] = (uint8_t)sb;
-        }
+        const float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        const uint32_t sb = fp8_scale_byte(
+            __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + row * ncols + col) =
+            fp8_codes4(v, fp8_inv_scale(sb));
+        if (lane_id() == 0) p.sy[fp8_scale_at(row, tile, fp8_groups(ncols))] = (uint8_t)sb;
       } else {
-        if (col >= ncols) continue;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          if (j0 + i * split >= hi) break;
-          const long at = (long)(m0 + j0 + i * split) * ncols + col;
-          float t = v[i];
-          if (p.bias != nullptr) t += bf2f(p.bias[(long)expert * p.N + col]);
-          if constexpr (EPI == kEpiResid) t += bf2f(p.resid[at]);
-          if constexpr (EPI == kEpiStoreF32)
-            static_cast<float*>(p.y)[at] = t;
-          else
-            static_cast<bf16*>(p.y)[at] = f2bf(t);
-        }
+        const long at = row * ncols + col;
+        const bool whole = col + 4 <= ncols && (ncols & 3) == 0;   // four columns, aligned together
+        if (p.bias != nullptr) add4(v, p.bias + (long)expert * p.N + col, whole, ncols - col);
+        if constexpr (EPI == kEpiResid) add4(v, p.resid + at, whole, ncols - col);
+        if constexpr (EPI == kEpiStoreF32)
+          store4(static_cast<float*>(p.y) + at, v, whole, ncols - col);
+        else
+          store4(static_cast<bf16*>(p.y) + at, v, whole, ncols - col);
       }
     }
   }
@@ -767,16 +808,19 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
   return cudaLaunchKernelEx(&cfg, k, ma, mb, mbh, msa, msb, msbh, p) == cudaSuccess ? 0 : 2;
 }
 
-// How many CTAs share a tile's k-blocks: the cluster size with the least time
-// in units of one k-block, rounds of the grid (two CTAs an SM) times the k-blocks of a CTA
-// plus what the exchange of the partial sums costs.
-inline int few_split(long tiles, int n_kblk, int slots)
+// How many CTAs share a tile's k-blocks: the cluster size with the least
+// time, counted in k-blocks: rounds of the grid times (the k-blocks of a CTA
+// + its set-up), plus what the exchange of the partial sums costs. resident[s]: the
+// clusters of s CTAs that run at once, which the layout of the SMs makes
+// fewer than the free places for some s (288 CTAs as clusters of 6 took two
+// rounds where 256 as clusters of 8 took one).
+inline int few_split(long tiles, int n_kblk, const int* resident)
 {
   int best = 1;
   long best_cost = -1;
-  for (int s = 1; s <= 8 && s <= n_kblk; ++s) {
-    const long rounds = (tiles * s + slots - 1) / slots;
-    const long cost = rounds * ((n_kblk + s - 1) / s + 4) + (s > 1 ? s : 0);
+  for (int s = 1; s <= kMaxSplit && s <= n_kblk; ++s) {
+    const long rounds = (tiles + resident[s] - 1) / resident[s];
+    const long cost = rounds * ((n_kblk + s - 1) / s + kFewSetUp) + (s > 1 ? s : 0);
     if (best_cost < 0 || cost < best_cost) {
       best = s;
       best_cost = cost;
@@ -821,20 +865,40 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::s
     return 2;
   auto k = gemm_fp8_few_kernel<MT, EPI>;
   if (!smem_attr_once(k, C::kSmem, attr_set)) return 2;
-  const int split = few_split((long)tiles * units, p.n_kblk, C::kPerSm * a.num_sms);
+  cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(split, tiles, units);
   cfg.blockDim = dim3(kThreadsFew);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attrs[2] = {};
   attrs[0].id = cudaLaunchAttributeClusterDimension;
-  attrs[0].val.clusterDim.x = split;
   attrs[0].val.clusterDim.y = 1;
   attrs[0].val.clusterDim.z = 1;
   attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attrs;
+  cfg.numAttrs = 1;
+  // clusters of each size that can be resident, asked once per device
+  static std::mutex mu;
+  static int resident_dev[64][kMaxSplit + 1];
+  int dev = 0, resident[kMaxSplit + 1];
+  if (cudaGetDevice(&dev) != cudaSuccess) return 2;
+  {
+    std::lock_guard<std::mutex> g(mu);
+    int* r = resident_dev[dev & 63];
+    for (int s = 1; s <= kMaxSplit; ++s) {
+      if (r[s] == 0) {
+        attrs[0].val.clusterDim.x = s;
+        cfg.gridDim = dim3(s);
+        if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0)
+          r[s] = std::max(1, C::kPerSm * a.num_sms / s / 2);
+      }
+      resident[s] = r[s];
+    }
+  }
+  const int split = few_split((long)tiles * units, p.n_kblk, resident);
+  attrs[0].val.clusterDim.x = split;
+  cfg.gridDim = dim3(split, tiles, units);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, k, mx, mw, msx, msw, p) == cudaSuccess ? 0 : 2;
 }
