@@ -432,9 +432,10 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 // accumulator is an output column and its columns are the activation rows.
 // The k-blocks of a tile are split over the CTAs of a cluster; their partial
 // sums meet in shared memory, each CTA adding (in rank order) and finishing
-// its share of the rows. Two CTAs fit an SM, which keeps ~200 KB of weights
-// in flight there.
-//   warp 0     TMA producer, one k-block a stage
+// its share of the rows. The runtime keeps one CTA with a TMEM allocation on
+// an SM, so a CTA rings ~200 KB of weights, two k-blocks a stage (one k-block
+// a stage: the issuer's ~200 cycles a stage showed).
+//   warp 0     TMA producer
 //   warp 1     MMA issuer
 //   warps 2-5  TMEM -> shared memory; then every warp: the sum over the
 //              cluster and the epilogue, a row a warp
@@ -443,27 +444,23 @@ constexpr int kThreadsFew = 192;
 constexpr int kFewRows = 128;       // rows up to which this form runs
 constexpr int kFewPrefetch = 4;     // k-blocks a CTA sends towards L2 ahead of its loads
 constexpr int kMaxSplit = 8;        // the portable cluster size
-constexpr int kFewSetUp = 4;        // a CTA's set-up, in k-blocks
 
 template <int MT, bool GU>
 struct FewCfg {
-  static constexpr int kA = GU ? 2 * kTileBytes : kTileBytes;
+  static constexpr int kNA = GU ? 2 : 1;
+  static constexpr int kKps = GU && MT >= 64 ? 1 : 2;       // k-blocks per stage
+  static constexpr int kA = kNA * kTileBytes;               // of one k-block
   static constexpr int kB = MT * 128;
-  static constexpr int kStage = kA + kB + 2048;            // + the scale tiles
-  static constexpr int kPerSm = GU && MT == 128 ? 1 : 2;   // 512 TMEM columns: alone on its SM
-  static constexpr int kStages = (kPerSm == 1 ? 4 : (114000 - 2048) / kStage);
+  static constexpr int kStage = kKps * (kA + kB) + 2048;    // + the scale tiles
+  static constexpr int kStages = (232448 - 1280) / kStage < 6 ? (232448 - 1280) / kStage : 6;
   static constexpr int kSmem = kStages * kStage + 1024 /*align*/ + 256 /*bars*/;
-  static constexpr int kAcc = GU ? 2 * MT : MT;            // accumulator columns
-  static constexpr int kSf = GU ? 12 : 8;                  // scale columns of a set, two sets
-  static constexpr int kCols = kAcc + 2 * kSf <= 32    ? 32
-                               : kAcc + 2 * kSf <= 64  ? 64
+  static constexpr int kAcc = kNA * MT;                     // accumulator columns
+  static constexpr int kSf = GU ? 12 : 8;                   // scale columns of a set, two sets
+  static constexpr int kCols = kAcc + 2 * kSf <= 64    ? 64
                                : kAcc + 2 * kSf <= 128 ? 128
                                : kAcc + 2 * kSf <= 256 ? 256
                                                        : 512;
-  static_assert(kStages >= 2 && kStages * kStage >= kAcc * 512, "the partial sums take the ring");
-  // two CTAs an SM share its 512 TMEM columns, and a third never fits beside
-  // them (its allocation would wait for theirs while their clusters wait for it)
-  static_assert(kPerSm == 1 ? kSmem > 116736 : kCols <= 256 && kSmem > 77824 && kSmem <= 115712, "");
+  static_assert(kStages >= 3 && kStages * kStage >= kAcc * 512, "the partial sums take the ring");
 };
 
 struct FewParams {
@@ -516,7 +513,7 @@ __device__ __forceinline__ void store4(float* dst, const float (&v)[4], bool who
 }
 
 template <int MT, int EPI>
-__global__ void __launch_bounds__(kThreadsFew, 2)
+__global__ void __launch_bounds__(kThreadsFew, 1)
     gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmX,
                         const __grid_constant__ CUtensorMap tmW,
                         const __grid_constant__ CUtensorMap tmSX,
@@ -533,6 +530,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::kStages,
                  accf = empty0 + 8 * C::kStages, drain = accf + 8;
 
+  griddep_launch();
   const uint32_t w = warp_id();
   const int split = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster is the x axis
   const int tile = blockIdx.y;
@@ -544,99 +542,119 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
   const int m0 = (p.seg_off[s_] / MT + ((int)blockIdx.z - p.unit_start[s_])) * MT;
   const int lo = max(m0, p.seg_off[s_]) - m0, hi = min(m0 + MT, p.seg_off[s_ + 1]) - m0;
   const int expert = p.seg_expert[s_];
-  const int kb0 = (int)((long)rank * p.n_kblk / split), kb1 = (int)((long)(rank + 1) * p.n_kblk / split);
+  // this CTA's stages of the tile, and their first k-block
+  const int n_st = (p.n_kblk + C::kKps - 1) / C::kKps;
+  const int st0 = rank * n_st / split, st1 = (rank + 1) * n_st / split;
   const int wrow = expert * p.N + tile * 128 * NA;
   const uint32_t base = smem_u32(smem);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full0 + 8 * s, 1);
-      mbar_init(empty0 + 8 * s, 1);
+  // stage i of this CTA (its empty barrier waited for by the caller)
+  auto load = [&](int i) {
+    const int s = i % C::kStages, kb = (st0 + i) * C::kKps;
+    const int nk = min(C::kKps, p.n_kblk - kb);
+    const uint32_t st = base + s * C::kStage, fb = full0 + 8 * s;
+    const bool sfs = i == 0 || (kb & 3) == 0;   // a scale tile serves its four k-blocks
+    if (elect_one()) {
+      mbar_arrive_expect_tx(fb, nk * (C::kA + C::kB) + (sfs ? (NA + 1) * kFp8SfTile : 0));
+#pragma unroll
+      for (int hk = 0; hk < C::kKps; ++hk) {
+        if (hk >= nk) break;
+#pragma unroll
+        for (int h = 0; h < NA; ++h)
+          tma_load_2d(st + (hk * NA + h) * kTileBytes, &tmW, (kb + hk) * 128, wrow + 128 * h, fb);
+        tma_load_2d(st + C::kKps * C::kA + hk * C::kB, &tmX, (kb + hk) * 128, m0, fb);
+      }
+      if (sfs) {
+        const uint32_t sf = st + C::kKps * (C::kA + C::kB);
+        tma_load_sf(sf, &tmSX, kb >> 2, m0 >> 7, fb);
+#pragma unroll
+        for (int h = 0; h < NA; ++h)
+          tma_load_sf(sf + (1 + h) * kFp8SfTile, &tmSW, kb >> 2,
+                      expert * p.sf_blk_expert + tile * NA + h, fb);
+      }
     }
-    mbar_init(accf, 1);
-    mbar_init(drain, 1);
-    fence_barrier_init();
-  }
-  if (w == 1) {
+    __syncwarp();
+  };
+
+  const int n_it = st1 - st0;
+  if (w == 0) {
+    if (elect_one()) {
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(full0 + 8 * s, 1);
+        mbar_init(empty0 + 8 * s, 1);
+      }
+      mbar_init(accf, 1);
+      mbar_init(drain, 1);
+      fence_barrier_init();
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmX);
+      tma_prefetch_desc(&tmSW);
+      tma_prefetch_desc(&tmSX);
+      // the weights' first tiles start towards L2 while the previous kernel
+      // still runs (a prefetch reads nothing into this CTA: were they being
+      // written, L2 holds the new bytes when the loads come)
+      for (int i = 0; i < min(kFewPrefetch, min(st1 * C::kKps, p.n_kblk) - st0 * C::kKps); ++i)
+        for (int h = 0; h < NA; ++h)
+          tma_prefetch_2d(&tmW, (st0 * C::kKps + i) * 128, wrow + 128 * h);
+    }
+    __syncwarp();
+    griddep_wait();
+    for (int i = 0; i < min(C::kStages, n_it); ++i) load(i);   // the ring is empty
+  } else if (w == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::kCols);
     tmem_relinquish();
-  }
-  if (w == 0 && lane_id() == 0) {
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmX);
-    tma_prefetch_desc(&tmSW);
-    tma_prefetch_desc(&tmSX);
-    // the weights' first tiles start towards L2 while the previous kernel
-    // still runs (a prefetch reads nothing into this CTA: were they being
-    // written, L2 holds the new bytes when the loads come)
-    const int pf = min(kb1, kb0 + kFewPrefetch);
-    for (int kb = kb0; kb < pf; ++kb)
-      for (int h = 0; h < NA; ++h) tma_prefetch_2d(&tmW, kb * 128, wrow + 128 * h);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  griddep_launch();
-  griddep_wait();
 
   if (w == 0) {
-    int it = 0;
-    for (int kb = kb0; kb < kb1; ++kb, ++it) {
-      const int s = it % C::kStages, ph = (it / C::kStages) & 1;
-      if (!warp_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) break;
-      const uint32_t st = base + s * C::kStage, fb = full0 + 8 * s;
-      const bool sfs = kb == kb0 || (kb & 3) == 0;   // a scale tile serves its four k-blocks
-      if (elect_one()) {
-        mbar_arrive_expect_tx(fb, C::kA + C::kB + (sfs ? (NA + 1) * kFp8SfTile : 0));
-#pragma unroll
-        for (int h = 0; h < NA; ++h)
-          tma_load_2d(st + h * kTileBytes, &tmW, kb * 128, wrow + 128 * h, fb);
-        tma_load_2d(st + C::kA, &tmX, kb * 128, m0, fb);
-        if (sfs) {
-          const uint32_t sf = st + C::kA + C::kB;
-          tma_load_sf(sf, &tmSX, kb >> 2, m0 >> 7, fb);
-#pragma unroll
-          for (int h = 0; h < NA; ++h)
-            tma_load_sf(sf + (1 + h) * kFp8SfTile, &tmSW, kb >> 2,
-                        expert * p.sf_blk_expert + tile * NA + h, fb);
-        }
-      }
-      __syncwarp();
+    int it = min(C::kStages, n_it);
+    for (; it < n_it; ++it) {
+      if (!warp_wait(empty0 + 8 * (it % C::kStages), (it / C::kStages & 1) ^ 1, p.err, kDevWaitEmpty))
+        break;
+      load(it);
     }
     for (int s = 0; s < C::kStages; ++s)   // every fill has landed before the CTA may exit
       if (it > s) warp_wait(full0 + 8 * s, ((it - 1 - s) / C::kStages) & 1, p.err, kDevWaitDrain);
   } else if (w == 1) {
     constexpr uint32_t idesc = idesc_e4m3(128, MT);
-    int it = 0;
     uint32_t set = 0;
     bool ok = true;
-    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+    for (int it = 0; it < n_it; ++it) {
       const int s = it % C::kStages, ph = (it / C::kStages) & 1;
       if (!warp_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
         ok = false;
         break;
       }
       tc_fence_after();
+      const int kb = (st0 + it) * C::kKps;
+      const int nk = min(C::kKps, p.n_kblk - kb);
       const uint32_t st = base + s * C::kStage;
-      if (it != 0 && (kb & 3) == 0) set ^= 1;
+      const bool sfs = it == 0 || (kb & 3) == 0;
+      set ^= sfs;
       const uint32_t sfx = tmem + C::kAcc + set * C::kSf, sfw = sfx + 4;
-      const uint32_t id = idesc | idesc_scale_byte(kb & 3);
-      const uint64_t ad = smem_desc_sw128(st), bd = smem_desc_sw128(st + C::kA);
+      const uint64_t ad = smem_desc_sw128(st), bd = smem_desc_sw128(st + C::kKps * C::kA);
       if (elect_one()) {
-        if (it == 0 || (kb & 3) == 0) {
-          const uint64_t sf = smem_desc_sf(st + C::kA + C::kB);
+        if (sfs) {
+          const uint64_t sf = smem_desc_sf(st + C::kKps * (C::kA + C::kB));
           sf_copy(sfx, sf);
 #pragma unroll
           for (int h = 0; h < NA; ++h) sf_copy(sfw + 4 * h, sf + (1 + h) * (kFp8SfTile >> 4));
         }
-        // K = 32 steps are 32 bytes, 2 descriptor units, apart
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int hk = 0; hk < C::kKps; ++hk) {
+          if (hk >= nk) break;
+          const uint32_t id = idesc | idesc_scale_byte((kb + hk) & 3);
+          // K = 32 steps are 32 bytes, 2 descriptor units, apart
 #pragma unroll
-          for (int h = 0; h < NA; ++h)
-            mma_e4m3(tmem + h * MT, ad + h * (kTileBytes >> 4) + k * 2, bd + k * 2, id, sfw + 4 * h,
-                     sfx, (it | k) != 0);
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int h = 0; h < NA; ++h)
+              mma_e4m3(tmem + h * MT, ad + (hk * NA + h) * (kTileBytes >> 4) + k * 2,
+                       bd + hk * (C::kB >> 4) + k * 2, id, sfw + 4 * h, sfx, (it | hk | k) != 0);
+        }
         mma_commit(empty0 + 8 * s);
       }
       __syncwarp();
@@ -649,6 +667,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2)
     warp_wait(drain, 0, p.err, kDevWaitDrain);
   }
 
+  if (w != 0) griddep_wait();
   float* part = reinterpret_cast<float*>(smem);   // [NA][MT rows][128 columns], over the ring
   const int wq = (int)(w & 3), n = wq * 32 + (int)lane_id();
   bool ok = true;
@@ -809,18 +828,17 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
 }
 
 // How many CTAs share a tile's k-blocks: the cluster size with the least
-// time, counted in k-blocks: rounds of the grid times (the k-blocks of a CTA
-// + its set-up), plus what the exchange of the partial sums costs. resident[s]: the
-// clusters of s CTAs that run at once, which the layout of the SMs makes
-// fewer than the free places for some s (288 CTAs as clusters of 6 took two
-// rounds where 256 as clusters of 8 took one).
-inline int few_split(long tiles, int n_kblk, const int* resident)
+// time, in nanoseconds as measured: rounds of the grid times (a CTA's stages
+// + its set-up and first loads), plus what the exchange of the partial sums
+// costs. resident[s]: the clusters of s CTAs that run at once, which the
+// layout of the SMs makes fewer than SMs / s for most s.
+inline int few_split(long tiles, int n_stages, int stage_ns, const int* resident)
 {
   int best = 1;
   long best_cost = -1;
-  for (int s = 1; s <= kMaxSplit && s <= n_kblk; ++s) {
+  for (int s = 1; s <= kMaxSplit && s <= n_stages; ++s) {
     const long rounds = (tiles + resident[s] - 1) / resident[s];
-    const long cost = rounds * ((n_kblk + s - 1) / s + kFewSetUp) + (s > 1 ? s : 0);
+    const long cost = rounds * ((n_stages + s - 1) / s * (long)stage_ns + 2500) + (s > 1 ? 400 + 50 * s : 0);
     if (best_cost < 0 || cost < best_cost) {
       best = s;
       best_cost = cost;
@@ -865,7 +883,6 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::s
     return 2;
   auto k = gemm_fp8_few_kernel<MT, EPI>;
   if (!smem_attr_once(k, C::kSmem, attr_set)) return 2;
-  cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreadsFew);
   cfg.dynamicSmemBytes = C::kSmem;
@@ -891,12 +908,13 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::s
         attrs[0].val.clusterDim.x = s;
         cfg.gridDim = dim3(s);
         if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0)
-          r[s] = std::max(1, C::kPerSm * a.num_sms / s / 2);
+          r[s] = std::max(1, a.num_sms / s / 2);
       }
       resident[s] = r[s];
     }
   }
-  const int split = few_split((long)tiles * units, p.n_kblk, resident);
+  const int split = few_split((long)tiles * units, (p.n_kblk + C::kKps - 1) / C::kKps,
+                              C::kKps * C::kNA * 160, resident);
   attrs[0].val.clusterDim.x = split;
   cfg.gridDim = dim3(split, tiles, units);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
