@@ -589,7 +589,9 @@ int u15c_mot_add_rms_norm_quant_fp8(u15c_stream stream, const void* x, const voi
   if (!fill_seg(&seg, seg_off, seg_expert, nseg, rows, n_experts, &err))
     return fail(U15C_EINVAL, "add_rms_norm_quant_fp8: " + err);
   if (rows == 0) return U15C_OK;
-  LAUNCH(launch_add_rms_norm_fp8(x, delta, w_stack, x_out, q, scale, rows, dim, eps, seg,
+  DevState* d = dev();
+  if (d == nullptr) return U15C_ECUDA;
+  LAUNCH(launch_add_rms_norm_fp8(x, delta, w_stack, x_out, q, scale, rows, dim, eps, seg, d->sms,
                                  ST(stream)),
          "add_rms_norm_quant_fp8");
 }
@@ -709,9 +711,10 @@ int u15c_mot_ffn_fp8(u15c_stream stream, const void* x, const void* delta,
   int rc = check_gemm_fp8(up);
   if (!rc) rc = check_gemm_fp8(down);
   if (rc || rows == 0) return rc;
-  if (dev() == nullptr) return U15C_ECUDA;
+  DevState* d = dev();
+  if (d == nullptr) return U15C_ECUDA;
   if (launch_add_rms_norm_fp8(x, delta, w_norm_stack, delta != nullptr ? y : nullptr, b + o.n,
-                              b + o.ns, rows, hidden, eps, seg, ST(stream)))
+                              b + o.ns, rows, hidden, eps, seg, d->sms, ST(stream)))
     return fail(U15C_ECUDA, "ffn_fp8: norm launch failed");
   rc = run_gemm_fp8(up, seg, ST(stream));
   return rc ? rc : run_gemm_fp8(down, seg, ST(stream));

@@ -4,6 +4,8 @@
 #include "u15_fp8.cuh"
 #include "u15_kernels.h"
 
+#include <algorithm>
+
 namespace u15 {
 
 namespace {
@@ -23,12 +25,16 @@ __device__ __forceinline__ float max16(float v)
   for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-__device__ __forceinline__ void unpack8f(const uint4& u, float (&v)[8])
+__device__ __forceinline__ void unpack8f(const uint4& u, float* v)
 {
-  const float2 a = unpack_bf2(u.x), b = unpack_bf2(u.y), c = unpack_bf2(u.z), d = unpack_bf2(u.w);
-  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
 }
-__device__ __forceinline__ uint4 pack8f(const float (&v)[8])
+__device__ __forceinline__ uint4 pack8f(const float* v)
 {
   return make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]),
                     pack_bf2(v[6], v[7]));
@@ -51,98 +57,198 @@ __device__ __forceinline__ int seg_expert_of(int row, const SegInfo& s)
 
 // ---------------------------------------------------------------------
 // s = bf16(x + delta); y = s / sqrt(mean(s^2) + eps) * w_e; q = e4m3(y).
-// One CTA per row, NT threads with KW runs of 8 columns each, kept packed in
-// registers between the sum of squares and the output (KW = 0: any width, the
-// row read again). Sums in f32, and y is rounded once, to e4m3. x_out may be
-// x or delta: every element is read and written by one thread.
+// NT threads take a row, KW runs of 16 columns each (eight lanes a block of
+// 128), and walk the rows with the grid's stride; a row stays in registers
+// between its sum of squares and its output. Sums in f32; s * w is exact
+// (two bf16), the reciprocal root correctly rounded, so y carries two f32
+// roundings ahead of its one to e4m3. x_out may be x or delta: every element
+// is read and written by one thread.
 // ---------------------------------------------------------------------
+
+// 1 / sqrt(v), rounded once: r = 1 / s and s = sqrt(v) are rounded, and their
+// exact residuals 1 - s r and v - s^2 (one fma each) give the next term of
+// 1 / sqrt(s^2 + d) = 1 / s - d / (2 s^3)
+__device__ __forceinline__ float rsqrt_exact(float v)
+{
+  const float s = __fsqrt_rn(v), r = __fdiv_rn(1.0f, s);
+  const float e = __fmaf_rn(-s, r, 1.0f), d = __fmaf_rn(-s, s, v);
+  return s == INFINITY ? 0.0f : __fmaf_rn(r, __fmaf_rn(-0.5f * d * r, r, e), r);
+}
+
+// threads of the norm resident on an SM
+constexpr int kNormThreads = 1024;
+
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 template <int NT, int KW>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT)
     add_norm_fp8_kernel(const bf16* x, const bf16* delta, const bf16* __restrict__ w, bf16* x_out,
-                        uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int dim, float eps,
-                        SegInfo seg)
+                        uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int rows, int dim,
+                        float eps, SegInfo seg)
+{
+  constexpr int kCta = NT < 128 ? 128 : NT, kRows = kCta / NT;   // rows a CTA takes at once
+  griddep_launch();
+  griddep_wait();
+  const int lane_in = threadIdx.x % NT, groups = fp8_groups(dim);
+  __shared__ float red[2][NT / 32];
+  int par = 0;
+  // every thread of the CTA runs the same number of rounds
+  for (long r0 = (long)blockIdx.x * kRows; r0 < rows; r0 += (long)gridDim.x * kRows, par ^= 1) {
+    const long row = r0 + threadIdx.x / NT;
+    const bool live = row < rows;
+    float2 t[KW][8];
+    float2 acc2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const int c = (k * NT + lane_in) * 16;
+      float* v = &t[k][0].x;
+      uint4 u[2] = {};
+      if (live && c < dim) {
+        const uint4* px = reinterpret_cast<const uint4*>(x + row * dim + c);
+        u[0] = px[0];
+        u[1] = px[1];
+      }
+      unpack8f(u[0], v);
+      unpack8f(u[1], v + 8);
+      if (delta != nullptr) {
+        if (live && c < dim) {
+          const uint4* pd = reinterpret_cast<const uint4*>(delta + row * dim + c);
+          float b[16];
+          unpack8f(pd[0], b);
+          unpack8f(pd[1], b + 8);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] += b[i];
+        }
+        u[0] = pack8f(v);
+        u[1] = pack8f(v + 8);
+        unpack8f(u[0], v);
+        unpack8f(u[1], v + 8);
+      }
+      if (x_out != nullptr && live && c < dim) {
+        uint4* po = reinterpret_cast<uint4*>(x_out + row * dim + c);
+        po[0] = u[0];
+        po[1] = u[1];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc2 = fma2(t[k][i], t[k][i], acc2);
+    }
+    float acc = wsum(acc2.x + acc2.y);
+    if constexpr (NT > 32) {
+      if (lane_id() == 0) red[par][warp_id()] = acc;
+      __syncthreads();
+      acc = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NT / 32; ++i) acc += red[par][i];
+    }
+    const float inv = rsqrt_exact(__fdiv_rn(acc, (float)dim) + eps);
+    const bf16* wr = w + (long)(live ? seg_expert_of((int)row, seg) : 0) * dim;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const int c = (k * NT + lane_in) * 16;
+      uint4 gw[2] = {};
+      if (c < dim) {
+        gw[0] = __ldg(reinterpret_cast<const uint4*>(wr + c));
+        gw[1] = __ldg(reinterpret_cast<const uint4*>(wr + c) + 1);
+      }
+      float2 g[8];
+      unpack8f(gw[0], &g[0].x);
+      unpack8f(gw[1], &g[4].x);
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t[k][i] = mul2(mul2(t[k][i], g[i]), make_float2(inv, inv));
+        m = fmaxf(m, fmaxf(fabsf(t[k][i].x), fabsf(t[k][i].y)));
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const uint32_t s = fp8_scale_byte(m);
+      const float f = fp8_inv_scale(s, m);
+      if (live && c < dim) {
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 a = mul2(t[k][2 * i], make_float2(f, f)),
+                       b = mul2(t[k][2 * i + 1], make_float2(f, f));
+          h[i] = __byte_perm(fp8_codes2(a.x, a.y), fp8_codes2(b.x, b.y), 0x5410);
+        }
+        *reinterpret_cast<uint4*>(q + row * dim + c) = make_uint4(h[0], h[1], h[2], h[3]);
+        if ((lane_id() & 7) == 0) scale[fp8_scale_at(row, c >> 7, groups)] = (uint8_t)s;
+      }
+    }
+  }
+}
+
+// The same for rows too wide for registers: one CTA a row, which it reads twice.
+__global__ void __launch_bounds__(512)
+    add_norm_wide_fp8_kernel(const bf16* x, const bf16* delta, const bf16* __restrict__ w, bf16* x_out,
+                             uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int dim, float eps,
+                             SegInfo seg)
 {
   griddep_launch();
   griddep_wait();
-  const int row = blockIdx.x;
-  const long base = (long)row * dim;
-  const bf16* wr = w + (long)seg_expert_of(row, seg) * dim;
+  const long row = blockIdx.x;
+  const bf16* wr = w + (long)seg_expert_of((int)row, seg) * dim;
   const int groups = fp8_groups(dim);
-  __shared__ float red[NT / 32];
-
-  // the row's run of 8 columns at c, the residual's sum rounded and stored
-  auto load = [&](int c) -> uint4 {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (c < dim) {
-      u = *reinterpret_cast<const uint4*>(x + base + c);
-      if (delta != nullptr) {
-        float a[8], b[8];
-        unpack8f(u, a);
-        unpack8f(*reinterpret_cast<const uint4*>(delta + base + c), b);
+  __shared__ float red[16];
+  auto load = [&](int c) {
+    uint4 u = *reinterpret_cast<const uint4*>(x + row * dim + c);
+    if (delta == nullptr) return u;
+    float a[8], b[8];
+    unpack8f(u, a);
+    unpack8f(*reinterpret_cast<const uint4*>(delta + row * dim + c), b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] += b[i];
-        u = pack8f(a);
-      }
-      if (x_out != nullptr) *reinterpret_cast<uint4*>(x_out + base + c) = u;
-    }
-    return u;
+    for (int i = 0; i < 8; ++i) a[i] += b[i];
+    return pack8f(a);
   };
-  auto squares = [&](const uint4& u, float acc) {
+  float acc = 0.0f;
+  for (int c = threadIdx.x * 8; c < dim; c += 512 * 8) {
+    const uint4 u = load(c);
+    if (x_out != nullptr) *reinterpret_cast<uint4*>(x_out + row * dim + c) = u;
     float t[8];
     unpack8f(u, t);
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc = __fmaf_rn(t[i], t[i], acc);
-    return acc;
-  };
-  auto rstd = [&](float acc) {
-    acc = wsum(acc);
-    if (lane_id() == 0) red[warp_id()] = acc;
-    __syncthreads();
-    float t = 0.0f;
+  }
+  acc = wsum(acc);
+  if (lane_id() == 0) red[warp_id()] = acc;
+  __syncthreads();
+  acc = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NT / 32; ++i) t += red[i];
-    return __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(t, (float)dim) + eps));
-  };
-  // all lanes of a warp call this together: the block's largest is a shuffle
-  auto out = [&](const uint4& u, int c, float inv) {
-    float t[8], g[8];
-    unpack8f(u, t);
-    unpack8f(c < dim ? __ldg(reinterpret_cast<const uint4*>(wr + c)) : make_uint4(0, 0, 0, 0), g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = c < dim ? t[i] * inv * g[i] : 0.0f;
-    const uint32_t s = fp8_scale_byte(max16(amax8(t)));
+  for (int i = 0; i < 16; ++i) acc += red[i];
+  const float inv = rsqrt_exact(__fdiv_rn(acc, (float)dim) + eps);
+  for (int c0 = 0; c0 < dim; c0 += 512 * 8) {
+    const int c = c0 + threadIdx.x * 8;
+    float t[8] = {}, g[8];
     if (c < dim) {
-      *reinterpret_cast<uint2*>(q + base + c) = fp8_codes8(t, fp8_inv_scale(s));
+      // the sum from where it was stored: x or delta may be that place
+      unpack8f(x_out != nullptr ? *reinterpret_cast<const uint4*>(x_out + row * dim + c) : load(c), t);
+      unpack8f(__ldg(reinterpret_cast<const uint4*>(wr + c)), g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = t[i] * g[i] * inv;
+    }
+    const float m = max16(amax8(t));
+    const uint32_t s = fp8_scale_byte(m);
+    if (c < dim) {
+      *reinterpret_cast<uint2*>(q + row * dim + c) = fp8_codes8(t, fp8_inv_scale(s, m));
       if ((lane_id() & 15) == 0) scale[fp8_scale_at(row, c >> 7, groups)] = (uint8_t)s;
-    }
-  };
-
-  if constexpr (KW > 0) {
-    uint4 u[KW];
-    float acc = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      u[k] = load((k * NT + threadIdx.x) * 8);
-      acc = squares(u[k], acc);
-    }
-    const float inv = rstd(acc);
-#pragma unroll
-    for (int k = 0; k < KW; ++k) out(u[k], (k * NT + threadIdx.x) * 8, inv);
-  } else {
-    float acc = 0.0f;
-    for (int c0 = 0; c0 < dim; c0 += NT * 8) acc = squares(load(c0 + threadIdx.x * 8), acc);
-    const float inv = rstd(acc);
-    // the sum again: from x_out where it was stored (x or delta may be it)
-    for (int c0 = 0; c0 < dim; c0 += NT * 8) {
-      const int c = c0 + threadIdx.x * 8;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (c < dim) {
-        if (x_out != nullptr)
-          u = *reinterpret_cast<const uint4*>(x_out + base + c);
-        else
-          u = load(c);
-      }
-      out(u, c, inv);
     }
   }
 }
@@ -176,9 +282,10 @@ __global__ void __launch_bounds__(256)
     const int c = c0 + k * 256;
     float t[8];
     unpack8f(u[k], t);
-    const uint32_t s = fp8_scale_byte(max16(amax8(t)));
+    const float m = max16(amax8(t));
+    const uint32_t s = fp8_scale_byte(m);
     if (c < cols) {
-      *reinterpret_cast<uint2*>(q + row * cols + c) = fp8_codes8(t, fp8_inv_scale(s));
+      *reinterpret_cast<uint2*>(q + row * cols + c) = fp8_codes8(t, fp8_inv_scale(s, m));
       if ((lane_id() & 15) == 0) scale[fp8_scale_at(row, c >> 7, groups)] = (uint8_t)s;
     }
   }
@@ -217,7 +324,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = fmaxf(m, red[i]);
   const uint32_t s = fp8_scale_byte(m);
-  const float inv = fp8_inv_scale(s);
+  const float inv = fp8_inv_scale(s, m);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + i * 16 + (threadIdx.x >> 4);
@@ -260,21 +367,41 @@ __global__ void __launch_bounds__(256)
 
 }  // namespace
 
+namespace {
+
+template <int NT, int KW>
+cudaError_t launch_norm(const bf16* x, const bf16* delta, const bf16* w, bf16* x_out, uint8_t* q,
+                        uint8_t* scale, int rows, int dim, float eps, const SegInfo& seg,
+                        int num_sms, cudaStream_t st)
+{
+  constexpr int kCta = NT < 128 ? 128 : NT, kRows = kCta / NT;
+  const int grid = std::min((rows + kRows - 1) / kRows, num_sms * (kNormThreads / kCta));
+  return launch_pdl(add_norm_fp8_kernel<NT, KW>, dim3(grid), dim3(kCta), st, x, delta, w, x_out, q,
+                    scale, rows, dim, eps, seg);
+}
+
+}  // namespace
+
 int launch_add_rms_norm_fp8(const void* x, const void* delta, const void* w, void* x_out,
                             uint8_t* q, uint8_t* scale, int rows, int dim, float eps,
-                            const SegInfo& seg, cudaStream_t st)
+                            const SegInfo& seg, int num_sms, cudaStream_t st)
 {
   if (rows <= 0) return 0;
   const bf16 *xb = static_cast<const bf16*>(x), *db = static_cast<const bf16*>(delta),
              *wb = static_cast<const bf16*>(w);
   bf16* ob = static_cast<bf16*>(x_out);
-  cudaError_t e;
-  if (dim <= 4096)
-    e = launch_pdl(add_norm_fp8_kernel<128, 4>, dim3(rows), dim3(128), st, xb, db, wb, ob, q,
-                   scale, dim, eps, seg);
-  else
-    e = launch_pdl(add_norm_fp8_kernel<256, 0>, dim3(rows), dim3(256), st, xb, db, wb, ob, q,
-                   scale, dim, eps, seg);
+  // the fewest threads that hold a row at up to 32 (wide rows: 48) columns each
+  const auto k = dim <= 512     ? launch_norm<32, 1>
+                 : dim <= 1024  ? launch_norm<32, 2>
+                 : dim <= 2048  ? launch_norm<128, 1>
+                 : dim <= 4096  ? launch_norm<128, 2>
+                 : dim <= 8192  ? launch_norm<256, 2>
+                 : dim <= 12288 ? launch_norm<256, 3>
+                                : nullptr;
+  const cudaError_t e =
+      k != nullptr ? k(xb, db, wb, ob, q, scale, rows, dim, eps, seg, num_sms, st)
+                   : launch_pdl(add_norm_wide_fp8_kernel, dim3(rows), dim3(512), st, xb, db, wb, ob,
+                                q, scale, dim, eps, seg);
   return e == cudaSuccess ? 0 : 2;
 }
 

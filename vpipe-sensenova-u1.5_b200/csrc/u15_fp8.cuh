@@ -45,42 +45,38 @@ __device__ __forceinline__ uint32_t fp8_scale_byte(float amax)
   const int s = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   return (uint32_t)max(s, 0);
 }
-// 2^(127 - s), a normal float for every s the rule gives (0 .. 248)
-__device__ __forceinline__ float fp8_inv_scale(uint32_t s) { return __uint_as_float((254u - s) << 23); }
+// 2^(127 - s), a normal float for every s the rule gives (0 .. 248), by which
+// a block's values are multiplied ahead of their rounding; 0 where the block
+// holds an Inf (amax never counts a NaN): Inf * 0 is NaN, so a value that is
+// not finite becomes the NaN code instead of saturating to 448, at no
+// instruction per value
+__device__ __forceinline__ float fp8_inv_scale(uint32_t s, float amax)
+{
+  return amax < INFINITY ? __uint_as_float((254u - s) << 23) : 0.0f;
+}
 // 2^(s - 127); s = 0 is 2^-127, a subnormal float
 __device__ __forceinline__ float fp8_scale_value(uint32_t s)
 {
   return s != 0 ? __uint_as_float(s << 23) : __uint_as_float(0x400000u);
 }
 
-// e4m3 codes of v[0..8) * inv as 8 bytes, v[0] lowest: rounded to nearest
-// even. v * 0 is NaN for an Inf (and for a NaN), so a value that is not
-// finite becomes the NaN code instead of saturating to 448.
+// two f32 values as two e4m3 codes, lo in the low byte: rounded to nearest even
+__device__ __forceinline__ uint32_t fp8_codes2(float lo, float hi)
+{
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+// e4m3 codes of v[0..8) * inv as 8 bytes, v[0] lowest
 __device__ __forceinline__ uint2 fp8_codes8(const float (&v)[8], float inv)
 {
   uint32_t h[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 f;
-    f.x = __fmaf_rn(v[2 * i], 0.0f, v[2 * i] * inv);
-    f.y = __fmaf_rn(v[2 * i + 1], 0.0f, v[2 * i + 1] * inv);
-    h[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-  }
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+  for (int i = 0; i < 4; ++i) h[i] = fp8_codes2(v[2 * i] * inv, v[2 * i + 1] * inv);
+  return make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
 }
-
 // the same for four values
 __device__ __forceinline__ uint32_t fp8_codes4(const float (&v)[4], float inv)
 {
-  uint32_t h[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float2 f;
-    f.x = __fmaf_rn(v[2 * i], 0.0f, v[2 * i] * inv);
-    f.y = __fmaf_rn(v[2 * i + 1], 0.0f, v[2 * i + 1] * inv);
-    h[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-  }
-  return h[0] | (h[1] << 16);
+  return __byte_perm(fp8_codes2(v[0] * inv, v[1] * inv), fp8_codes2(v[2] * inv, v[3] * inv), 0x5410);
 }
 
 // two e4m3 values as floats (exact)

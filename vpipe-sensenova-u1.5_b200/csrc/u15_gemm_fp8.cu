@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           if (!warp_wait(amax0 + 8 * wq, lt & 1, p.err, kDevWaitAccFull)) break;
           m = fmaxf(m, am[(wh ^ 1) * 128 + r_in]);
           const uint32_t sb = fp8_scale_byte(m);
-          const float inv = fp8_inv_scale(sb);
+          const float inv = fp8_inv_scale(sb, m);
           if (row_ok) {
             uint8_t* yrow = static_cast<uint8_t*>(p.y) + (long)row * nout + ti.nb * 128;
 #pragma unroll
@@ -722,11 +722,13 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
       }
       const long row = m0 + j;
       if constexpr (EPI == kEpiSwigluFp8) {
-        const float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-        const uint32_t sb = fp8_scale_byte(
-            __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+        float m = 0.0f;   // never NaN: fmaxf drops them
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[i]));
+        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+        const uint32_t sb = fp8_scale_byte(m);
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + row * ncols + col) =
-            fp8_codes4(v, fp8_inv_scale(sb));
+            fp8_codes4(v, fp8_inv_scale(sb, m));
         if (lane_id() == 0) p.sy[fp8_scale_at(row, tile, fp8_groups(ncols))] = (uint8_t)sb;
       } else {
         const long at = row * ncols + col;
