@@ -591,8 +591,8 @@ int u15c_mot_add_rms_norm_quant_fp8(u15c_stream stream, const void* x, const voi
   if (rows == 0) return U15C_OK;
   DevState* d = dev();
   if (d == nullptr) return U15C_ECUDA;
-  LAUNCH(launch_add_rms_norm_fp8(x, delta, w_stack, x_out, q, scale, rows, dim, eps, seg, d->sms,
-                                 ST(stream)),
+  LAUNCH(launch_add_rms_norm_fp8(x, delta, w_stack, x_out, q, scale, rows, dim, eps, seg, d->err,
+                                 d->sms, ST(stream)),
          "add_rms_norm_quant_fp8");
 }
 
@@ -714,7 +714,7 @@ int u15c_mot_ffn_fp8(u15c_stream stream, const void* x, const void* delta,
   DevState* d = dev();
   if (d == nullptr) return U15C_ECUDA;
   if (launch_add_rms_norm_fp8(x, delta, w_norm_stack, delta != nullptr ? y : nullptr, b + o.n,
-                              b + o.ns, rows, hidden, eps, seg, d->sms, ST(stream)))
+                              b + o.ns, rows, hidden, eps, seg, d->err, d->sms, ST(stream)))
     return fail(U15C_ECUDA, "ffn_fp8: norm launch failed");
   rc = run_gemm_fp8(up, seg, ST(stream));
   return rc ? rc : run_gemm_fp8(down, seg, ST(stream));

@@ -5,6 +5,7 @@
 #include "u15_kernels.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace u15 {
 
@@ -60,23 +61,28 @@ __device__ __forceinline__ int seg_expert_of(int row, const SegInfo& s)
 // NT threads take a row, KW runs of 16 columns each (eight lanes a block of
 // 128), and walk the rows with the grid's stride; a row stays in registers
 // between its sum of squares and its output. Sums in f32; s * w is exact
-// (two bf16), the reciprocal root correctly rounded, so y carries two f32
-// roundings ahead of its one to e4m3. x_out may be x or delta: every element
+// (two bf16), the mean and the reciprocal root are off by about half a unit, so
+// y carries little more than one f32 rounding ahead of its one to e4m3. x_out may be x or delta: every element
 // is read and written by one thread.
 // ---------------------------------------------------------------------
 
-// 1 / sqrt(v), rounded once: r = 1 / s and s = sqrt(v) are rounded, and their
-// exact residuals 1 - s r and v - s^2 (one fma each) give the next term of
-// 1 / sqrt(s^2 + d) = 1 / s - d / (2 s^3)
-__device__ __forceinline__ float rsqrt_exact(float v)
+// 1 / sqrt(v) to within about half a unit: the hardware's approximation and one
+// Newton step whose residual 1 - v r^2 is formed without rounding v r (an fma
+// gives what the product lost)
+__device__ __forceinline__ float rsqrt_newton(float v)
 {
-  const float s = __fsqrt_rn(v), r = __fdiv_rn(1.0f, s);
-  const float e = __fmaf_rn(-s, r, 1.0f), d = __fmaf_rn(-s, s, v);
-  return s == INFINITY ? 0.0f : __fmaf_rn(r, __fmaf_rn(-0.5f * d * r, r, e), r);
+  const float r = rsqrtf(v);
+  const float h = v * r, l = __fmaf_rn(v, r, -h);
+  const float e = __fmaf_rn(-l, r, __fmaf_rn(-h, r, 1.0f));
+  return v == INFINITY ? 0.0f : __fmaf_rn(0.5f * r, e, r);
+}
+// acc / dim the same way: inv_dim = 1 / dim as a rounded value and its rest
+__device__ __forceinline__ float mean_of(float acc, float2 inv_dim)
+{
+  return __fmaf_rn(acc, inv_dim.x, acc * inv_dim.y);
 }
 
-// threads of the norm resident on an SM
-constexpr int kNormThreads = 1024;
+constexpr int kNormSmem = 200 * 1024;   // bytes of row stages on an SM
 
 // two f32 operations in one instruction
 __device__ __forceinline__ float2 mul2(float2 a, float2 b)
@@ -98,42 +104,112 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
   return r;
 }
 
+// Rows come through shared memory, two stages of a CTA's rows each (x, then
+// delta), copied by the bulk engine: a round's rows are refilled with those two
+// rounds on as soon as every thread has them in registers. Loads into
+// registers left the memory idle between a row's loads and its output (4096 x
+// 4096 without a residual 15.3 us).
+// max(m, |a|, |b|) in one instruction (NaN is dropped)
+__device__ __forceinline__ float max_abs3(float m, float a, float b)
+{
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
+  return r;
+}
+
+// CTAs of a form on an SM: the registers that its row, gains and temporaries
+// take (46 / 72 / 104 for 1 / 2 / 3 runs); the grid is no larger, since
+// CTAs that wait for a place find the row stages empty (4096 x 4096: 7
+// a SM 12.8 us, 12 14.7)
 template <int NT, int KW>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT)
+constexpr int norm_ctas()
+{
+  return (KW == 1 ? 1280 : KW == 2 ? 896 : 512) / (NT < 128 ? 128 : NT);
+}
+
+template <int NT, int KW>
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT, norm_ctas<NT, KW>())
     add_norm_fp8_kernel(const bf16* x, const bf16* delta, const bf16* __restrict__ w, bf16* x_out,
                         uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int rows, int dim,
-                        float eps, SegInfo seg)
+                        float2 inv_dim, float eps, SegInfo seg, unsigned* err)
 {
   constexpr int kCta = NT < 128 ? 128 : NT, kRows = kCta / NT;   // rows a CTA takes at once
-  griddep_launch();
-  griddep_wait();
-  const int lane_in = threadIdx.x % NT, groups = fp8_groups(dim);
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(8) uint64_t bars[2];
   __shared__ float red[2][NT / 32];
-  int par = 0;
-  // every thread of the CTA runs the same number of rounds
-  for (long r0 = (long)blockIdx.x * kRows; r0 < rows; r0 += (long)gridDim.x * kRows, par ^= 1) {
-    const long row = r0 + threadIdx.x / NT;
-    const bool live = row < rows;
+  griddep_launch();
+  const uint32_t bar0 = smem_u32(bars), ring0 = smem_u32(ring);
+  const int half = kRows * dim * 2, stage = delta != nullptr ? 2 * half : half;
+  const int step = gridDim.x * kRows;
+  auto fill = [&](int s, int r) {   // one thread: rows [r, r + kRows) into stage s
+    const uint32_t n = (uint32_t)min(kRows, rows - r) * dim * 2;
+    mbar_arrive_expect_tx(bar0 + 8 * s, delta != nullptr ? 2 * n : n);
+    bulk_load(ring0 + s * stage, x + (long)r * dim, n, bar0 + 8 * s);
+    if (delta != nullptr) bulk_load(ring0 + s * stage + half, delta + (long)r * dim, n, bar0 + 8 * s);
+  };
+  const int first = blockIdx.x * kRows;
+  if (threadIdx.x == 0) {
+    mbar_init(bar0, 1);
+    mbar_init(bar0 + 8, 1);
+    fence_barrier_init();
+    griddep_wait();
+    if (first < rows) fill(0, first);
+    if (first + step < rows) fill(1, first + step);
+  }
+  __syncthreads();
+  griddep_wait();
+  // this thread's columns: k NT 16 + c0, and where their block's byte is
+  const int sub = NT < 128 ? threadIdx.x / NT : 0, c0 = (threadIdx.x % NT) * 16;
+  const int groups = fp8_groups(dim);
+  bool col[KW];
+  int sb_at[KW];
+#pragma unroll
+  for (int k = 0; k < KW; ++k) {
+    const int c = k * NT * 16 + c0;
+    col[k] = c < dim;
+    sb_at[k] = (c >> 9) * kFp8SfTile + ((c >> 7) & 3);
+  }
+  uint32_t it = 0;
+  int cur = -1;
+  bool ok = true;
+  uint4 gw[KW][2] = {};   // the gains of expert `cur`, read again only where it changes
+  // every thread of the CTA runs the same number of rounds (rows + 2 step < 2^31)
+  for (int r0 = first; r0 < rows; r0 += step, ++it) {
+    const int st = it & 1, row = r0 + sub;
+    const bool live = kRows == 1 || row < rows;
+    const int e = live ? seg_expert_of(row, seg) : cur;
+    if (e != cur) {
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const uint4* pw = reinterpret_cast<const uint4*>(w + (long)e * dim + k * NT * 16 + c0);
+        if (col[k]) {
+          gw[k][0] = __ldg(pw);
+          gw[k][1] = __ldg(pw + 1);
+        }
+      }
+      cur = e;
+    }
+    ok = mbar_wait(bar0 + 8 * st, (it >> 1) & 1, err, kDevWaitFull) && ok;
+    const uint8_t* src = ring + st * stage + (sub * dim + c0) * 2;
+    const long at = (long)row * dim + c0;
     float2 t[KW][8];
     float2 acc2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < KW; ++k) {
-      const int c = (k * NT + lane_in) * 16;
       float* v = &t[k][0].x;
       uint4 u[2] = {};
-      if (live && c < dim) {
-        const uint4* px = reinterpret_cast<const uint4*>(x + row * dim + c);
-        u[0] = px[0];
-        u[1] = px[1];
+      const bool here = live && col[k];
+      if (here) {
+        u[0] = *reinterpret_cast<const uint4*>(src + k * NT * 32);
+        u[1] = *reinterpret_cast<const uint4*>(src + k * NT * 32 + 16);
       }
       unpack8f(u[0], v);
       unpack8f(u[1], v + 8);
       if (delta != nullptr) {
-        if (live && c < dim) {
-          const uint4* pd = reinterpret_cast<const uint4*>(delta + row * dim + c);
+        if (here) {
           float b[16];
-          unpack8f(pd[0], b);
-          unpack8f(pd[1], b + 8);
+          unpack8f(*reinterpret_cast<const uint4*>(src + k * NT * 32 + half), b);
+          unpack8f(*reinterpret_cast<const uint4*>(src + k * NT * 32 + half + 16), b + 8);
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] += b[i];
         }
@@ -142,55 +218,59 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
         unpack8f(u[0], v);
         unpack8f(u[1], v + 8);
       }
-      if (x_out != nullptr && live && c < dim) {
-        uint4* po = reinterpret_cast<uint4*>(x_out + row * dim + c);
+      if (x_out != nullptr && here) {
+        uint4* po = reinterpret_cast<uint4*>(x_out + at + k * NT * 16);
         po[0] = u[0];
         po[1] = u[1];
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc2 = fma2(t[k][i], t[k][i], acc2);
+      for (int i = 0; i < 8; ++i) acc2 = __ffma2_rn(t[k][i], t[k][i], acc2);
     }
     float acc = wsum(acc2.x + acc2.y);
+    if (NT > 32 && lane_id() == 0) red[st][warp_id()] = acc;
+    __syncthreads();   // every thread has its columns: the stage is free
+    if (threadIdx.x == 0 && r0 + 2 * step < rows) fill(st, r0 + 2 * step);
     if constexpr (NT > 32) {
-      if (lane_id() == 0) red[par][warp_id()] = acc;
-      __syncthreads();
       acc = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NT / 32; ++i) acc += red[par][i];
+      for (int i = 0; i < NT / 32; ++i) acc += red[st][i];
     }
-    const float inv = rsqrt_exact(__fdiv_rn(acc, (float)dim) + eps);
-    const bf16* wr = w + (long)(live ? seg_expert_of((int)row, seg) : 0) * dim;
+    const float inv = rsqrt_newton(mean_of(acc, inv_dim) + eps);
+    uint8_t* const srow = scale + fp8_scale_at(row, 0, groups);
 #pragma unroll
     for (int k = 0; k < KW; ++k) {
-      const int c = (k * NT + lane_in) * 16;
-      uint4 gw[2] = {};
-      if (c < dim) {
-        gw[0] = __ldg(reinterpret_cast<const uint4*>(wr + c));
-        gw[1] = __ldg(reinterpret_cast<const uint4*>(wr + c) + 1);
-      }
       float2 g[8];
-      unpack8f(gw[0], &g[0].x);
-      unpack8f(gw[1], &g[4].x);
+      unpack8f(gw[k][0], &g[0].x);
+      unpack8f(gw[k][1], &g[4].x);
       float m = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        t[k][i] = mul2(mul2(t[k][i], g[i]), make_float2(inv, inv));
-        m = fmaxf(m, fmaxf(fabsf(t[k][i].x), fabsf(t[k][i].y)));
+        t[k][i] = __fmul2_rn(t[k][i], g[i]);
+        m = max_abs3(m, t[k][i].x, t[k][i].y);
       }
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      // the largest |y| is the largest |s w| times 1 / root (rounding keeps
+      // order), and the block's power of two goes into the same factor: y is
+      // rounded as if it had been formed first
+      m *= inv;
       const uint32_t s = fp8_scale_byte(m);
-      const float f = fp8_inv_scale(s, m);
-      if (live && c < dim) {
-        uint32_t h[4];
+      float f = inv * fp8_inv_scale(s, m);
+      if (f == INFINITY) {   // an all but zero block: two steps
+        f = fp8_inv_scale(s, m);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 a = mul2(t[k][2 * i], make_float2(f, f)),
-                       b = mul2(t[k][2 * i + 1], make_float2(f, f));
-          h[i] = __byte_perm(fp8_codes2(a.x, a.y), fp8_codes2(b.x, b.y), 0x5410);
-        }
-        *reinterpret_cast<uint4*>(q + row * dim + c) = make_uint4(h[0], h[1], h[2], h[3]);
-        if ((lane_id() & 7) == 0) scale[fp8_scale_at(row, c >> 7, groups)] = (uint8_t)s;
+        for (int i = 0; i < 8; ++i) t[k][i] = __fmul2_rn(t[k][i], make_float2(inv, inv));
+      }
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = __fmul2_rn(t[k][2 * i], make_float2(f, f)),
+                     b = __fmul2_rn(t[k][2 * i + 1], make_float2(f, f));
+        h[i] = __byte_perm(fp8_codes2(a.x, a.y), fp8_codes2(b.x, b.y), 0x5410);
+      }
+      if (live && col[k] && ok) {
+        *reinterpret_cast<uint4*>(q + at + k * NT * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+        if ((lane_id() & 7) == 0) srow[sb_at[k]] = (uint8_t)s;
       }
     }
   }
@@ -199,8 +279,8 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
 // The same for rows too wide for registers: one CTA a row, which it reads twice.
 __global__ void __launch_bounds__(512)
     add_norm_wide_fp8_kernel(const bf16* x, const bf16* delta, const bf16* __restrict__ w, bf16* x_out,
-                             uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int dim, float eps,
-                             SegInfo seg)
+                             uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int dim,
+                             float2 inv_dim, float eps, SegInfo seg)
 {
   griddep_launch();
   griddep_wait();
@@ -233,7 +313,7 @@ __global__ void __launch_bounds__(512)
   acc = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc += red[i];
-  const float inv = rsqrt_exact(__fdiv_rn(acc, (float)dim) + eps);
+  const float inv = rsqrt_newton(mean_of(acc, inv_dim) + eps);
   for (int c0 = 0; c0 < dim; c0 += 512 * 8) {
     const int c = c0 + threadIdx.x * 8;
     float t[8] = {}, g[8];
@@ -369,22 +449,43 @@ __global__ void __launch_bounds__(256)
 
 namespace {
 
+float2 inverse_of(int dim)
+{
+  const double inv = 1.0 / dim;
+  return make_float2((float)inv, (float)(inv - (double)(float)inv));
+}
+
 template <int NT, int KW>
 cudaError_t launch_norm(const bf16* x, const bf16* delta, const bf16* w, bf16* x_out, uint8_t* q,
                         uint8_t* scale, int rows, int dim, float eps, const SegInfo& seg,
-                        int num_sms, cudaStream_t st)
+                        unsigned* err, int num_sms, cudaStream_t st)
 {
+  static std::atomic<uint64_t> attr_set;
   constexpr int kCta = NT < 128 ? 128 : NT, kRows = kCta / NT;
-  const int grid = std::min((rows + kRows - 1) / kRows, num_sms * (kNormThreads / kCta));
-  return launch_pdl(add_norm_fp8_kernel<NT, KW>, dim3(grid), dim3(kCta), st, x, delta, w, x_out, q,
-                    scale, rows, dim, eps, seg);
+  constexpr int kMost = 2 * 2 * kRows * NT * KW * 16 * 2;   // two stages of x and delta
+  const auto k = add_norm_fp8_kernel<NT, KW>;
+  if (!smem_attr_once(k, kMost, attr_set)) return cudaErrorInvalidValue;
+  const int smem = 2 * kRows * dim * 2 * (delta != nullptr ? 2 : 1);
+  const int per_sm = std::max(1, std::min(norm_ctas<NT, KW>(), kNormSmem / smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(std::min((rows + kRows - 1) / kRows, num_sms * per_sm));
+  cfg.blockDim = dim3(kCta);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k, x, delta, w, x_out, q, scale, rows, dim, inverse_of(dim), eps, seg,
+                            err);
 }
 
 }  // namespace
 
 int launch_add_rms_norm_fp8(const void* x, const void* delta, const void* w, void* x_out,
                             uint8_t* q, uint8_t* scale, int rows, int dim, float eps,
-                            const SegInfo& seg, int num_sms, cudaStream_t st)
+                            const SegInfo& seg, unsigned* err, int num_sms, cudaStream_t st)
 {
   if (rows <= 0) return 0;
   const bf16 *xb = static_cast<const bf16*>(x), *db = static_cast<const bf16*>(delta),
@@ -399,9 +500,9 @@ int launch_add_rms_norm_fp8(const void* x, const void* delta, const void* w, voi
                  : dim <= 12288 ? launch_norm<256, 3>
                                 : nullptr;
   const cudaError_t e =
-      k != nullptr ? k(xb, db, wb, ob, q, scale, rows, dim, eps, seg, num_sms, st)
+      k != nullptr ? k(xb, db, wb, ob, q, scale, rows, dim, eps, seg, err, num_sms, st)
                    : launch_pdl(add_norm_wide_fp8_kernel, dim3(rows), dim3(512), st, xb, db, wb, ob,
-                                q, scale, dim, eps, seg);
+                                q, scale, dim, inverse_of(dim), eps, seg);
   return e == cudaSuccess ? 0 : 2;
 }
 

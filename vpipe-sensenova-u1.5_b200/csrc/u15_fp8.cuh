@@ -203,6 +203,17 @@ __device__ __forceinline__ void tma_load_sf_pair(uint32_t smem_dst, const CUtens
       : "memory");
 }
 
+// untiled copy of `bytes` (a multiple of 16, both ends 16-byte aligned) to this
+// CTA's shared memory, counted on its mbarrier
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes,
+                                          uint32_t bar)
+{
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
 // L2 prefetch of a tile (no shared memory, no completion to wait for)
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int x, int y)
 {

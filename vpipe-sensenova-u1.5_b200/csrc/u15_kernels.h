@@ -146,7 +146,7 @@ int gemm_fp8(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::str
 // u15_fp8.cu
 int launch_add_rms_norm_fp8(const void* x, const void* delta, const void* w, void* x_out,
                             uint8_t* q, uint8_t* scale, int rows, int dim, float eps,
-                            const SegInfo& seg, int num_sms, cudaStream_t st);
+                            const SegInfo& seg, unsigned* err, int num_sms, cudaStream_t st);
 int launch_quant_rows_fp8(const void* x, uint8_t* q, uint8_t* scale, int rows, int cols,
                           cudaStream_t st);
 int launch_quant_weight_fp8(const void* w, uint8_t* q, uint8_t* scale, int n_experts, int N, int K,
