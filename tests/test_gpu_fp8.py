@@ -305,6 +305,55 @@ def test_repeats_bit_identical(ops):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+def torch_values(q, s, rows, cols):
+    """A quantised tensor's values in float64 on the device."""
+    at = torch.from_numpy(F.places(rows, cols)).cuda()
+    f = torch.exp2(s[at].double() - 127).repeat_interleave(128, 1)[:, :cols]
+    return q.view(torch.float8_e4m3fn).reshape(rows, cols).double() * f
+
+
+def random_quantised(ops, rows, cols, seed, std):
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = (std * torch.randn(rows, cols, generator=g, device="cuda")).bfloat16()
+    q, s = u8(rows * cols), ops.fp8_scale(rows, cols)
+    ops.quant_rows_fp8(x, q, s, rows, cols)
+    return q, s, torch_values(q, s, rows, cols)
+
+
+@pytest.mark.parametrize("M,K,N,segs", [
+    (2100, 640, 4096, [(0, 2100, 0)]),                         # a part-empty last round: half-width tiles
+    (1800, 512, 6144, [(0, 77, 0), (77, 1800, 1)]),            # several rounds, an odd boundary
+    (3000, 384, 2176, [(0, 250, 1), (250, 251, 0), (251, 1600, 1), (1600, 3000, 0)]),
+    (1030, 272, 8192, [(0, 320, 0), (320, 1030, 1)])])
+@pytest.mark.parametrize("epi", [STORE, RESID, SWIGLU])
+def test_many_tiles(ops, M, K, N, segs, epi):
+    """More tiles than CTA pairs: the accumulators' shared columns, the scale
+    sets' turns over tiles of odd group counts, and the last round."""
+    if epi == SWIGLU:
+        N -= N % 256                                            # whole gate and up blocks
+    xq, xs, x = random_quantised(ops, M, K, 1, 1.0)
+    W = [random_quantised(ops, N, K, 2 + e, 0.05) for e in range(2)]
+    wq, ws = torch.cat([w[0] for w in W]).view(2, N, K), torch.cat([w[1] for w in W])
+    cols = N // 2 if epi == SWIGLU else N
+    r = torch.randn(M, N, device="cuda").bfloat16() if epi == RESID else None
+    y = torch.empty(M, cols, dtype=torch.bfloat16, device="cuda")
+    ops.mot_linear_fp8(xq, xs, wq, ws, segs, y, M, K, N, epilogue=epi, resid=r)
+    ops.sync()
+    t = torch.cat([x[a:b] @ W[e][2].T for a, b, e in segs])
+    S = torch.cat([x[a:b].abs() @ W[e][2].abs().T for a, b, e in segs])
+    err = F.sum_error(S, K) + 2.0 ** -23 * t.abs()
+    if epi == SWIGLU:
+        g, u = t.view(M, -1, 2, 128).unbind(2)
+        eg, eu = err.view(M, -1, 2, 128).unbind(2)
+        silu = g / (1 + torch.exp(-g))
+        t = (silu * u).flatten(1)
+        err = (1.1 * eg * (u.abs() + eu) + silu.abs() * eu).flatten(1) + 2.0 ** -20 * t.abs()
+    if epi == RESID:
+        t = t + r.double()
+        err = err + 2.0 ** -23 * t.abs()
+    assert ((y.double() - t).abs() <= err + 2.0 ** -8 * t.abs()).all()
+
+
 # ------------------------------------------------------------------ SwiGLU
 def swiglu_ref(xq, xs, W, M, K, segs):
     """silu(gate) * up of every row, and what f32 sums may be off by there."""

@@ -21,7 +21,8 @@ using bf16 = __nv_bfloat16;
 // Many rows: a CTA pair (tcgen05 cta_group::2) computes 256 x 256 tiles.
 //   warp 0     TMA producer (both CTAs): per stage two k-blocks of 128
 //              columns, 128 rows of A and 128 of B a CTA, and the packed
-//              scale tiles of their group: the CTA's 128 rows of A, all 256 of B
+//              scale tiles of their group: the two that the CTA's 128 rows of A
+//              lie in, all 256 rows of B
 //   warp 1     MMA issuer (leader): copies the stage's scales to TMEM, then
 //              eight MMAs of K = 32, the block's scale byte in the descriptor
 //   warps 2-9  epilogue, two a TMEM lane quadrant, half the columns each
@@ -37,7 +38,7 @@ constexpr int kStageBytes = 2 * kKps * kTileBytes + 2048;   // operands, then th
 constexpr int kSmemPair = kStg * kStageBytes + 1024 /*align*/ + 2048 /*amax*/ + 256 /*bars*/;
 constexpr int kThreadsPair = 320;
 constexpr int kAccStep = 224;                  // accumulator 1 starts 32 columns early
-constexpr int kSfCol = 480;                    // two sets of 4 + 8 scale columns, 16 apart
+constexpr int kSfCol = 480;                    // two sets of 8 + 8 scale columns
 
 struct PairParams {
   int M, N, K;
@@ -67,15 +68,19 @@ __device__ __forceinline__ PairTile pair_tile(const PairParams& p, int t)
     t = p.n_full + (h >> 1);
     r.half = h & 1;
   }
-  // units (256-row blocks of one segment) run fastest: a round of the
-  // schedule reads few columns of B, and A stays in L2
+  // units (256 rows of one segment, from its first row rounded down to 64) run
+  // fastest: a round of the schedule reads few columns of B, and A stays in L2.
+  // Rows from a multiple of 64 on begin at the first or third scale column of
+  // their packed tile, so the four of a CTA's rows are taken from there on into
+  // the next tile's columns. (Blocks of 256 rows of the whole pass would
+  // need one scale tile, and a unit more where a segment straddles one.)
   const int unit = t % p.n_units;
   r.nb = t / p.n_units;
   int s = 0;
 #pragma unroll 1
   for (int k = 1; k < p.nseg; ++k)
     if (unit >= p.unit_start[k]) s = k;
-  r.m0 = (p.seg_off[s] / 256 + (unit - p.unit_start[s])) * 256;
+  r.m0 = (p.seg_off[s] & ~63) + (unit - p.unit_start[s]) * 256;
   r.row_lo = max(r.m0, p.seg_off[s]);
   r.row_hi = min(r.m0 + 256, p.seg_off[s + 1]);
   r.expert = p.seg_expert[s];
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
                        (half ? 128 * ti.half + 64 * (int)rank : 128 * (int)rank);
       const int sblk = ti.expert * p.sf_blk_expert + ti.nb * 2 + (half ? ti.half : 0);
       const uint32_t tx = kTileBytes + (half ? kTileBytes / 2 : kTileBytes);
-      const uint32_t tx_sf = half ? 2 * kFp8SfTile : 3 * kFp8SfTile;
+      const uint32_t tx_sf = half ? 3 * kFp8SfTile : 4 * kFp8SfTile;
       const CUtensorMap *mb = half ? &tmBh : &tmB, *msb = half ? &tmSBh : &tmSB;
       for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
         const uint32_t s = it % kStg, ph = (it / kStg) & 1;
@@ -222,7 +227,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           if (sfs) {
             const uint32_t sf = st + 2 * kKps * kTileBytes;
             tma_load_sf_pair(sf, &tmSA, kb >> 2, arow >> 7, fb);
-            tma_load_sf_pair(sf + kFp8SfTile, msb, kb >> 2, sblk, fb);
+            tma_load_sf_pair(sf + 2 * kFp8SfTile, msb, kb >> 2, sblk, fb);
           }
 #pragma unroll
           for (int hk = 0; hk < kKps; ++hk) {
@@ -259,6 +264,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
         if (lt > 0 && !warp_wait_cluster_probe(accr, (lt - 1) & 1, p.err, kDevWaitAccEmpty)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (lt & 1) * kAccStep;
+        const uint32_t a_col = (pair_tile(p, t).m0 >> 5) & 3;   // of the unit's first row: 0 or 2
         for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
           const uint32_t s = it % kStg, ph = (it / kStg) & 1;
           if (!warp_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
@@ -269,14 +275,15 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           const int nk = min(kKps, p.n_kblk - kb);
           const uint32_t st = base + s * kStageBytes;
           if ((kb & 3) == 0) sf_set ^= 1;
-          const uint32_t sfa = tmem_base + kSfCol + sf_set * 16, sfb = sfa + 4;
+          const uint32_t sfa = tmem_base + kSfCol + sf_set * 16, sfb = sfa + 8;
           const uint64_t ad = smem_desc_sw128(st), bd = smem_desc_sw128(st + kKps * kTileBytes);
           if (elect_one()) {
             if ((kb & 3) == 0) {
               const uint64_t sf = smem_desc_sf(st + 2 * kKps * kTileBytes);
               sf_copy_pair(sfa, sf);
-              sf_copy_pair(sfb, sf + (kFp8SfTile >> 4));
-              if (!half) sf_copy_pair(sfb + 4, sf + 2 * (kFp8SfTile >> 4));
+              if (a_col) sf_copy_pair(sfa + 4, sf + (kFp8SfTile >> 4));
+              sf_copy_pair(sfb, sf + 2 * (kFp8SfTile >> 4));
+              if (!half) sf_copy_pair(sfb + 4, sf + 3 * (kFp8SfTile >> 4));
             }
 #pragma unroll
             for (int hk = 0; hk < kKps; ++hk) {
@@ -286,7 +293,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 mma_e4m3_pair(d_tmem, ad + hk * (kTileBytes >> 4) + k * 2,
-                              bd + hk * (kTileBytes >> 4) + k * 2, id, sfa, sfb,
+                              bd + hk * (kTileBytes >> 4) + k * 2, id, sfa + a_col, sfb,
                               ((kb + hk) | k) != 0);
             }
             mma_commit_pair_mc(empty0 + 8 * s, 0x3);
@@ -775,7 +782,7 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
     p.seg_expert[s] = seg.expert[s];
     p.unit_start[s] = p.n_units;
     if (seg.off[s + 1] > seg.off[s])
-      p.n_units += (seg.off[s + 1] + 255) / 256 - seg.off[s] / 256;
+      p.n_units += (seg.off[s + 1] - (seg.off[s] & ~63) + 255) / 256;
   }
   p.seg_off[seg.nseg] = seg.off[seg.nseg];
   p.unit_start[seg.nseg] = p.n_units;
@@ -791,7 +798,7 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
                  wblks = (uint64_t)p.sf_blk_expert * a.n_experts, xblks = (a.M + 127) / 128;
   if (make_tma_2d(&ma, a.xq, a.M, a.K, 128, 1, err) || make_tma_2d(&mb, a.wq, wrows, a.K, 128, 1, err) ||
       make_tma_2d(&mbh, a.wq, wrows, a.K, 64, 1, err) ||
-      make_tma_fp8_scales(&msa, a.sx, xblks, groups, 1, err) ||
+      make_tma_fp8_scales(&msa, a.sx, xblks, groups, 2, err) ||
       make_tma_fp8_scales(&msb, a.sw, wblks, groups, 2, err) ||
       make_tma_fp8_scales(&msbh, a.sw, wblks, groups, 1, err))
     return 2;
