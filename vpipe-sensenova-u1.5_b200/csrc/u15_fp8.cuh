@@ -214,6 +214,22 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
+// 32 bytes of one lane in one store: whole sectors, where two 16-byte stores
+// send two half-filled ones (a lane owns a row here, so lanes do not share them)
+__device__ __forceinline__ void store32b(void* p, const uint32_t (&v)[8])
+{
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void load32b(const void* p, uint32_t (&v)[8])
+{
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+                 "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
 // L2 prefetch of a tile (no shared memory, no completion to wait for)
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int x, int y)
 {

@@ -93,14 +93,17 @@ __device__ __forceinline__ float swiglu1(float g, float u)
   return __fdividef(g, 1.0f + expf(-g)) * u;
 }
 
+// 32 columns of one row; columns >= ncols dropped
 __device__ __forceinline__ void store32(bf16* dst, const float (&v)[32], int col0, int ncols)
 {
-  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-    uint4* d4 = reinterpret_cast<uint4*>(dst);
+  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      d4[q] = make_uint4(pack_bf2(v[q * 8 + 0], v[q * 8 + 1]), pack_bf2(v[q * 8 + 2], v[q * 8 + 3]),
-                         pack_bf2(v[q * 8 + 4], v[q * 8 + 5]), pack_bf2(v[q * 8 + 6], v[q * 8 + 7]));
+    for (int q = 0; q < 2; ++q) {
+      uint32_t o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = pack_bf2(v[q * 16 + 2 * i], v[q * 16 + 2 * i + 1]);
+      store32b(dst + q * 16, o);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
@@ -109,10 +112,14 @@ __device__ __forceinline__ void store32(bf16* dst, const float (&v)[32], int col
 }
 __device__ __forceinline__ void store32(float* dst, const float (&v)[32], int col0, int ncols)
 {
-  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      reinterpret_cast<float4*>(dst)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    for (int q = 0; q < 4; ++q) {
+      uint32_t o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(v[q * 8 + i]);
+      store32b(dst + q * 8, o);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
@@ -121,13 +128,17 @@ __device__ __forceinline__ void store32(float* dst, const float (&v)[32], int co
 }
 __device__ __forceinline__ void add32(float (&v)[32], const bf16* src, int col0, int ncols)
 {
-  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(src) & 31) == 0) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint4 u = reinterpret_cast<const uint4*>(src)[q];
-      const float2 a = unpack_bf2(u.x), b = unpack_bf2(u.y), c = unpack_bf2(u.z), d = unpack_bf2(u.w);
-      v[q * 8 + 0] += a.x; v[q * 8 + 1] += a.y; v[q * 8 + 2] += b.x; v[q * 8 + 3] += b.y;
-      v[q * 8 + 4] += c.x; v[q * 8 + 5] += c.y; v[q * 8 + 6] += d.x; v[q * 8 + 7] += d.y;
+    for (int q = 0; q < 2; ++q) {
+      uint32_t u[8];
+      load32b(src + q * 16, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 a = unpack_bf2(u[i]);
+        v[q * 16 + 2 * i] += a.x;
+        v[q * 16 + 2 * i + 1] += a.y;
+      }
     }
   } else {
 #pragma unroll
@@ -375,6 +386,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           const float inv = fp8_inv_scale(sb, m);
           if (row_ok) {
             uint8_t* yrow = static_cast<uint8_t*>(p.y) + (long)row * nout + ti.nb * 128;
+            const bool whole_sectors = (reinterpret_cast<uintptr_t>(p.y) & 31) == 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               uint2 c[4];
@@ -385,9 +397,14 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
                 for (int j = 0; j < 8; ++j) v[j] = h[i][q * 8 + j];
                 c[q] = fp8_codes8(v, inv);
               }
-              uint4* d = reinterpret_cast<uint4*>(yrow + run[i] * 32);
-              d[0] = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
-              d[1] = make_uint4(c[2].x, c[2].y, c[3].x, c[3].y);
+              const uint32_t o[8] = {c[0].x, c[0].y, c[1].x, c[1].y, c[2].x, c[2].y, c[3].x, c[3].y};
+              if (whole_sectors) {
+                store32b(yrow + run[i] * 32, o);
+              } else {
+                uint4* d = reinterpret_cast<uint4*>(yrow + run[i] * 32);
+                d[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+              }
             }
             if (wh == 0) p.sy[fp8_scale_at(row, ti.nb, fp8_groups(nout))] = (uint8_t)sb;
           }
