@@ -84,31 +84,6 @@ __device__ __forceinline__ float mean_of(float acc, float2 inv_dim)
 
 constexpr int kNormSmem = 200 * 1024;   // bytes of row stages on an SM
 
-// two f32 operations in one instruction
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
-{
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "mov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-
-// Rows come through shared memory, two stages of a CTA's rows each (x, then
-// delta), copied by the bulk engine: a round's rows are refilled with those two
-// rounds on as soon as every thread has them in registers. Loads into
-// registers left the memory idle between a row's loads and its output (4096 x
-// 4096 without a residual 15.3 us).
 // max(m, |a|, |b|) in one instruction (NaN is dropped)
 __device__ __forceinline__ float max_abs3(float m, float a, float b)
 {

@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace u15 {
 
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 //              cluster and the epilogue, a row a warp
 // ---------------------------------------------------------------------
 constexpr int kThreadsFew = 192;
-constexpr int kFewRows = 128;       // rows up to which this form runs
+constexpr int kFewRows = 1024;      // rows up to which this form is considered
 constexpr int kFewPrefetch = 4;     // k-blocks a CTA sends towards L2 ahead of its loads
 constexpr int kMaxSplit = 8;        // the portable cluster size
 
@@ -717,54 +718,80 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
 
   if (ok) {
     // a warp finishes whole rows, four columns a lane: the sum over the
-    // cluster in rank order, and a row's largest needs no other warp
+    // cluster in rank order, and a row's largest needs no other warp. A step's
+    // loads are all in flight together: R rows from up to Q CTAs (row by row,
+    // 128 rows of an unsplit tile took 5 us; four rows from two CTAs at a time,
+    // eight CTAs' sums 2 us more)
+    constexpr int kWarps = kThreadsFew / 32;
     const uint32_t own = smem_u32(part) + lane_id() * 16;
     const int ncols = GU ? p.N / 2 : p.N, col = tile * 128 + (int)lane_id() * 4;
-    auto total = [&](int at) {
-      float4 v[8], t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int step = kWarps * split;
+    auto finish = [&](auto r_, auto q_) {
+      constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
+      for (int j0 = lo + rank + (int)w * split; j0 < hi; j0 += R * step) {
+        float4 v[Q][NA][R] = {};
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-        v[q] = q < split ? ld_cluster4(mapa_shared(own, q) + at * 512) : t;
+        for (int q = 0; q < Q; ++q) {
+          if (q >= split) break;
+          const uint32_t from = mapa_shared(own, q);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        t.x += v[q].x;
-        t.y += v[q].y;
-        t.z += v[q].z;
-        t.w += v[q].w;
+          for (int h = 0; h < NA; ++h)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+              if (j0 + i * step < hi) v[q][h][i] = ld_cluster4(from + (h * MT + j0 + i * step) * 512);
+        }
+        float4 t[NA][R];
+#pragma unroll
+        for (int h = 0; h < NA; ++h)
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            t[h][i] = v[0][h][i];
+#pragma unroll
+            for (int q = 1; q < Q; ++q) {
+              t[h][i].x += v[q][h][i].x;
+              t[h][i].y += v[q][h][i].y;
+              t[h][i].z += v[q][h][i].z;
+              t[h][i].w += v[q][h][i].w;
+            }
+          }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (j0 + i * step >= hi) break;
+          float v[4] = {t[0][i].x, t[0][i].y, t[0][i].z, t[0][i].w};
+          if constexpr (GU) {
+            v[0] = swiglu1(v[0], t[1][i].x);
+            v[1] = swiglu1(v[1], t[1][i].y);
+            v[2] = swiglu1(v[2], t[1][i].z);
+            v[3] = swiglu1(v[3], t[1][i].w);
+          }
+          const long row = m0 + j0 + i * step;
+          if constexpr (EPI == kEpiSwigluFp8) {
+            float m = 0.0f;   // never NaN: fmaxf drops them
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m = fmaxf(m, fabsf(v[k]));
+            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            const uint32_t sb = fp8_scale_byte(m);
+            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + row * ncols + col) =
+                fp8_codes4(v, fp8_inv_scale(sb, m));
+            if (lane_id() == 0) p.sy[fp8_scale_at(row, tile, fp8_groups(ncols))] = (uint8_t)sb;
+          } else {
+            const long at = row * ncols + col;
+            const bool whole = col + 4 <= ncols && (ncols & 3) == 0;   // four columns, aligned together
+            if (p.bias != nullptr) add4(v, p.bias + (long)expert * p.N + col, whole, ncols - col);
+            if constexpr (EPI == kEpiResid) add4(v, p.resid + at, whole, ncols - col);
+            if constexpr (EPI == kEpiStoreF32)
+              store4(static_cast<float*>(p.y) + at, v, whole, ncols - col);
+            else
+              store4(static_cast<bf16*>(p.y) + at, v, whole, ncols - col);
+          }
+        }
       }
-      return t;
     };
-    for (int j = lo + rank + (int)w * split; j < hi; j += (kThreadsFew / 32) * split) {
-      float4 t = total(j);
-      float v[4] = {t.x, t.y, t.z, t.w};
-      if constexpr (GU) {
-        t = total(MT + j);
-        v[0] = swiglu1(v[0], t.x);
-        v[1] = swiglu1(v[1], t.y);
-        v[2] = swiglu1(v[2], t.z);
-        v[3] = swiglu1(v[3], t.w);
-      }
-      const long row = m0 + j;
-      if constexpr (EPI == kEpiSwigluFp8) {
-        float m = 0.0f;   // never NaN: fmaxf drops them
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[i]));
-        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-        const uint32_t sb = fp8_scale_byte(m);
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + row * ncols + col) =
-            fp8_codes4(v, fp8_inv_scale(sb, m));
-        if (lane_id() == 0) p.sy[fp8_scale_at(row, tile, fp8_groups(ncols))] = (uint8_t)sb;
-      } else {
-        const long at = row * ncols + col;
-        const bool whole = col + 4 <= ncols && (ncols & 3) == 0;   // four columns, aligned together
-        if (p.bias != nullptr) add4(v, p.bias + (long)expert * p.N + col, whole, ncols - col);
-        if constexpr (EPI == kEpiResid) add4(v, p.resid + at, whole, ncols - col);
-        if constexpr (EPI == kEpiStoreF32)
-          store4(static_cast<float*>(p.y) + at, v, whole, ncols - col);
-        else
-          store4(static_cast<bf16*>(p.y) + at, v, whole, ncols - col);
-      }
-    }
+    using std::integral_constant;
+    if (split <= 2)
+      finish(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else
+      finish(integral_constant<int, 1>{}, integral_constant<int, kMaxSplit>{});
   }
 
   tc_fence_before();
@@ -853,30 +880,93 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
   return cudaLaunchKernelEx(&cfg, k, ma, mb, mbh, msa, msb, msbh, p) == cudaSuccess ? 0 : 2;
 }
 
-// How many CTAs share a tile's k-blocks: the cluster size with the least
-// time, in nanoseconds as measured: rounds of the grid times (a CTA's stages
-// + its set-up and first loads), plus what the exchange of the partial sums
-// costs. resident[s]: the clusters of s CTAs that run at once, which the
-// layout of the SMs makes fewer than SMs / s for most s.
-inline int few_split(long tiles, int n_stages, int stage_ns, const int* resident)
+// Row units of height h over the segments: blocks of h rows of the whole pass
+// (aligned) or of a segment from its first row rounded down to 64.
+inline int few_units(const SegInfo& seg, int h)
 {
-  int best = 1;
-  long best_cost = -1;
+  int n = 0;
+  for (int s = 0; s < seg.nseg; ++s)
+    if (seg.off[s + 1] > seg.off[s]) n += (seg.off[s + 1] + h - 1) / h - seg.off[s] / h;
+  return n;
+}
+inline int pair_units(const SegInfo& seg)
+{
+  int n = 0;
+  for (int s = 0; s < seg.nseg; ++s)
+    if (seg.off[s + 1] > seg.off[s]) n += (seg.off[s + 1] - (seg.off[s] & ~63) + 255) / 256;
+  return n;
+}
+
+// The few-row form's cluster size (how many CTAs share a tile's k-blocks) with
+// the least time, and that time in nanoseconds as measured: rounds of the grid times (a
+// CTA's stages + its set-up and first loads), plus what the exchange of the
+// partial sums costs. resident[s]: the clusters of s CTAs that run at once,
+// which the layout of the SMs makes fewer than SMs / s for most s.
+struct FewPlan {
+  int split = 1;
+  long ns = -1;
+};
+inline FewPlan few_plan(long tiles, int n_stages, int stage_ns, int round_ns, const int* resident)
+{
+  FewPlan best;
   for (int s = 1; s <= kMaxSplit && s <= n_stages; ++s) {
     const long rounds = (tiles + resident[s] - 1) / resident[s];
-    const long cost = rounds * ((n_stages + s - 1) / s * (long)stage_ns + 2500) + (s > 1 ? 400 + 50 * s : 0);
-    if (best_cost < 0 || cost < best_cost) {
-      best = s;
-      best_cost = cost;
-    }
+    const long ns = rounds * ((n_stages + s - 1) / s * (long)stage_ns + round_ns) + (s > 1 ? 400 + 50 * s : 0);
+    if (best.ns < 0 || ns < best.ns) best = FewPlan{s, ns};
   }
   return best;
 }
 
+// Clusters of each size that can be resident, asked once per kernel and device.
 template <int MT, int EPI>
-int launch_few(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+const int* few_resident(int num_sms)
 {
+  using C = FewCfg<MT, EPI == kEpiSwiglu || EPI == kEpiSwigluFp8>;
   static std::atomic<uint64_t> attr_set;
+  static std::mutex mu;
+  static int resident_dev[64][kMaxSplit + 1];
+  auto k = gemm_fp8_few_kernel<MT, EPI>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || !smem_attr_once(k, C::kSmem, attr_set)) return nullptr;
+  std::lock_guard<std::mutex> g(mu);
+  int* r = resident_dev[dev & 63];
+  if (r[0] != 0) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreadsFew);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  for (int s = 1; s <= kMaxSplit; ++s) {
+    attr[0].val.clusterDim.x = s;
+    cfg.gridDim = dim3(s);
+    if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0)
+      r[s] = std::max(1, num_sms / s / 2);
+  }
+  r[0] = 1;   // the entries are there
+  return r;
+}
+
+template <int MT, int EPI>
+FewPlan few_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* resident)
+{
+  constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
+  using C = FewCfg<MT, GU>;
+  const long tiles = (long)(GU ? a.N / 256 : (a.N + 127) / 128) * few_units(seg, MT);
+  // a k-block of 128 weight rows: 160 ns, or 400 with 128 activation rows
+  // beside them; a round's set-up, first loads and epilogue: 2.5 us and 20 ns a row
+  const int stage_ns = C::kKps * C::kNA * (MT <= 64 ? 160 : 400);
+  return few_plan(tiles, (fp8_blocks(a.K) + C::kKps - 1) / C::kKps, stage_ns, 2500 + 20 * MT,
+                  resident);
+}
+
+template <int MT, int EPI>
+int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cudaStream_t st,
+               std::string* err)
+{
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   using C = FewCfg<MT, GU>;
   FewParams p{};
@@ -907,44 +997,41 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::s
       make_tma_fp8_scales(&msx, a.sx, (a.M + 127) / 128, groups, 1, err) ||
       make_tma_fp8_scales(&msw, a.sw, (uint64_t)p.sf_blk_expert * a.n_experts, groups, 1, err))
     return 2;
-  auto k = gemm_fp8_few_kernel<MT, EPI>;
-  if (!smem_attr_once(k, C::kSmem, attr_set)) return 2;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreadsFew);
+  cfg.gridDim = dim3(plan.split, tiles, units);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attrs[2] = {};
   attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = plan.split;
   attrs[0].val.clusterDim.y = 1;
   attrs[0].val.clusterDim.z = 1;
   attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attrs;
-  cfg.numAttrs = 1;
-  // clusters of each size that can be resident, asked once per device
-  static std::mutex mu;
-  static int resident_dev[64][kMaxSplit + 1];
-  int dev = 0, resident[kMaxSplit + 1];
-  if (cudaGetDevice(&dev) != cudaSuccess) return 2;
-  {
-    std::lock_guard<std::mutex> g(mu);
-    int* r = resident_dev[dev & 63];
-    for (int s = 1; s <= kMaxSplit; ++s) {
-      if (r[s] == 0) {
-        attrs[0].val.clusterDim.x = s;
-        cfg.gridDim = dim3(s);
-        if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0)
-          r[s] = std::max(1, a.num_sms / s / 2);
-      }
-      resident[s] = r[s];
-    }
-  }
-  const int split = few_split((long)tiles * units, (p.n_kblk + C::kKps - 1) / C::kKps,
-                              C::kKps * C::kNA * 160, resident);
-  attrs[0].val.clusterDim.x = split;
-  cfg.gridDim = dim3(split, tiles, units);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k, mx, mw, msx, msw, p) == cudaSuccess ? 0 : 2;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_few_kernel<MT, EPI>, mx, mw, msx, msw, p) == cudaSuccess
+             ? 0
+             : 2;
+}
+
+template <int MT, int EPI>
+int launch_few_or_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+{
+  const int* resident = few_resident<MT, EPI>(a.num_sms);
+  if (resident == nullptr) return 2;
+  const FewPlan few = few_plan_of<MT, EPI>(a, seg, resident);
+  if (MT == 128) {
+    // 256 rows a tile against 128: the pairs' time is their rounds times 700 ns
+    // a stage (512 x 4096 x 12288: pairs 38 us, this form 40; 256 rows: 37 and
+    // 23; 256 x 24576 x 4096 SwiGLU: 30 and 57)
+    const long tiles = (long)pair_units(seg) * ((a.N + 255) / 256);
+    const long rounds = (tiles + a.num_sms / 2 - 1) / (a.num_sms / 2);
+    const long pair_ns = rounds * ((fp8_blocks(a.K) + kKps - 1) / kKps) * 700 + 5500;
+    if (pair_ns <= few.ns) return launch_pair<EPI>(a, seg, st, err);
+  }
+  return launch_few<MT, EPI>(a, seg, few, st, err);
 }
 
 template <int EPI>
@@ -952,10 +1039,10 @@ int launch_rows(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
 {
   const int tiles = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8 ? a.N / 256 : (a.N + 127) / 128;
   if (a.M > kFewRows || tiles > 65535) return launch_pair<EPI>(a, seg, st, err);
-  if (a.M <= 16) return launch_few<16, EPI>(a, seg, st, err);
-  if (a.M <= 32) return launch_few<32, EPI>(a, seg, st, err);
-  if (a.M <= 64) return launch_few<64, EPI>(a, seg, st, err);
-  return launch_few<128, EPI>(a, seg, st, err);
+  if (a.M <= 16) return launch_few_or_pair<16, EPI>(a, seg, st, err);
+  if (a.M <= 32) return launch_few_or_pair<32, EPI>(a, seg, st, err);
+  if (a.M <= 64) return launch_few_or_pair<64, EPI>(a, seg, st, err);
+  return launch_few_or_pair<128, EPI>(a, seg, st, err);
 }
 
 }  // namespace
