@@ -524,6 +524,7 @@ typedef struct u15c_config {
 } u15c_config;
 
 #define U15C_MODEL_INT8 1u /* also bind the W8A8 twin of every projection */
+#define U15C_MODEL_FP8 2u  /* also bind the e4m3 twin of every projection (one device) */
 
 /* tensor ids for u15c_model_bind, the 13 per-expert tensors of
  * src/u15-weights.cc:539-578 */
@@ -638,6 +639,7 @@ int u15c_kv_write(u15c_kv* kv, u15c_stream stream, int layer, int which_v, const
 
 #define U15C_FWD_INT8 1u /* W8A8 projections (i8_gemm) */
 #define U15C_FWD_SAGE 2u /* Sage int8-QK on the bidirectional pass */
+#define U15C_FWD_FP8 4u  /* e4m3 projections, a scale per block of 128 (not with _INT8) */
 
 /* The Sage tier's `dense_layers` (vpipe::genai::sage::Config, set through
  * MetalOps::set_sage, src/u15-metal-ops.cc:789-814, and honoured by

@@ -11,6 +11,7 @@
 //   down  [E][H][I]
 //   ln_in, ln_post [E][H]; norms [E][4][64] = q_norm, q_norm_hw, k_norm, k_norm_hw
 //   (INT8) the same four matrices as per-output-channel int8 plus f32 scales
+//   (FP8) the same four as e4m3 with a packed scale byte per 128 x 128 block
 // The GEMM's TMA maps tile these row-major buffers into 128-byte-swizzled
 // shared-memory tiles; no further repacking pays at these shapes.
 //
@@ -18,6 +19,7 @@
 // one logical->physical page table shared by all layers.
 #include "u15_capi_internal.h"
 #include "u15_common.cuh"
+#include "u15_fp8.cuh"
 
 #include <algorithm>
 #include <cstring>
@@ -47,6 +49,9 @@ struct LayerW {
   float* o_s = nullptr;
   float* gu_s = nullptr;
   float* down_s = nullptr;
+  // e4m3 twins and their packed scales (u15_fp8.cuh)
+  uint8_t *qkv_f8 = nullptr, *o_f8 = nullptr, *gu_f8 = nullptr, *down_f8 = nullptr;
+  uint8_t *qkv_fs = nullptr, *o_fs = nullptr, *gu_fs = nullptr, *down_fs = nullptr;
 };
 
 // ---------------------------------------------------------------------
@@ -153,6 +158,11 @@ struct u15c_model {
   float* rsin = nullptr;
   int8_t* x8 = nullptr;
   float* s_tok = nullptr;
+  // fp8 models: the quantised activations' scales (codes in x8), and the
+  // quantised SwiGLU rows
+  uint8_t* x_fs = nullptr;
+  uint8_t* h_f8 = nullptr;
+  uint8_t* h_fs = nullptr;
   void* sage_ws = nullptr;
   size_t sage_ws_bytes = 0;
   bf16* io = nullptr;   // layer_forward_host staging
@@ -247,6 +257,11 @@ struct u15c_model {
     rc |= alloc(&rsin, (size_t)n * 128 * 4, scratch_allocs);
     rc |= alloc(&x8, n * maxk, scratch_allocs);
     rc |= alloc(&s_tok, (size_t)n * 4, scratch_allocs);
+    if (flags & U15C_MODEL_FP8) {
+      rc |= alloc(&x_fs, u15::fp8_scale_bytes(n, (int)maxk), scratch_allocs);
+      rc |= alloc(&h_f8, n * I, scratch_allocs);
+      rc |= alloc(&h_fs, u15::fp8_scale_bytes(n, (int)I), scratch_allocs);
+    }
     rc |= alloc(&io, n * H * 2, scratch_allocs);
     sage_ws_bytes = u15::sage_bytes(cfg.heads, cfg.kv_heads, n, tk);
     rc |= alloc(reinterpret_cast<uint8_t**>(&sage_ws), sage_ws_bytes, scratch_allocs);
@@ -418,6 +433,11 @@ int layer_impl(u15c_model* m, cudaStream_t st, int li, bf16* x_all, int M,
   // the Sage tier leaves a prefix of the stack on the bf16 attention
   // (sdpa_steel's `sage_layer >= dense_layers`, src/u15-metal-ops.cc:852-855)
   if (li < m->sage_dense_layers) flags &= ~U15C_FWD_SAGE;
+  const bool f8 = (flags & U15C_FWD_FP8) != 0;
+  if (i8 && f8) return fail(U15C_EINVAL, "a pass runs W8A8 or fp8, not both");
+  if (f8 && L.qkv_f8 == nullptr)
+    return fail(U15C_EINVAL, "fp8 requested but the model has no e4m3 twins "
+                             "(create with U15C_MODEL_FP8 and call u15c_model_finalize)");
   if (i8 && L.qkv8 == nullptr)
     return fail(U15C_EINVAL, "W8A8 requested but the model has no int8 twins "
                              "(create with U15C_MODEL_INT8 and call u15c_model_finalize)");
@@ -509,8 +529,43 @@ int layer_impl(u15c_model* m, cudaStream_t st, int li, bf16* x_all, int M,
     return r ? fail(U15C_ECUDA, "rms_norm launch failed") : U15C_OK;
   };
 
+  // fp8: the norms quantise (the residual's addition stays in the products'
+  // epilogues, as in the bf16 layer), the SwiGLU product quantises its rows, and the
+  // attention's output is quantised by a pass of its own
+  auto norm8 = [&](const bf16* w) -> int {
+    u15::DevState* d = u15::dev();
+    if (d == nullptr) return U15C_ECUDA;
+    const int r = u15::launch_add_rms_norm_fp8(x, nullptr, w, nullptr,
+                                               reinterpret_cast<uint8_t*>(m->x8), m->x_fs, Mr, H,
+                                               (float)c.eps, seg, d->err, d->sms, st);
+    return r ? fail(U15C_ECUDA, "rms_norm (fp8) launch failed") : U15C_OK;
+  };
+  auto gemm8 = [&](const uint8_t* xq, const uint8_t* xs, int K, const uint8_t* w,
+                   const uint8_t* ws, int N, int epi, void* y, uint8_t* ys) -> int {
+    u15::GemmFp8Args a;
+    a.xq = xq;
+    a.sx = xs;
+    a.wq = w;
+    a.sw = ws;
+    a.n_experts = E;
+    a.M = Mr;
+    a.K = K;
+    a.N = N;
+    a.epilogue = epi;
+    a.resid = epi == u15::kEpiResid ? x : nullptr;
+    a.y = y;
+    a.sy = ys;
+    return u15::run_gemm_fp8(a, seg, st);
+  };
+  uint8_t* const xf = reinterpret_cast<uint8_t*>(m->x8);
+
   // ---- attention half (src/u15-backbone.cc:191-235) ----
-  if (parts & kPartPre) {
+  if ((parts & kPartPre) && f8) {
+    if ((rc = norm8(L.ln_in))) return rc;
+    if ((rc = gemm8(xf, m->x_fs, H, L.qkv_f8, L.qkv_fs, m->qkv_n(), u15::kEpiStore,
+                    m->qkv + (long)r0 * m->qkv_n(), nullptr)))
+      return rc;
+  } else if (parts & kPartPre) {
     if ((rc = norm(L.ln_in))) return rc;
     if ((rc = gemm(m->xn, H, L.qkv, L.qkv8, L.qkv_s, m->qkv_n(), u15::kEpiStore,
                    m->qkv + (long)r0 * m->qkv_n(), fuse_q)))
@@ -579,6 +634,15 @@ int layer_impl(u15c_model* m, cudaStream_t st, int li, bf16* x_all, int M,
     }
   }
   if (!(parts & kPartPost)) return U15C_OK;
+  if (f8) {
+    if (u15::launch_quant_rows_fp8(m->attn + (long)r0 * m->qd(), xf, m->x_fs, Mr, m->qd(), st))
+      return fail(U15C_ECUDA, "quant_rows (fp8) launch failed");
+    if ((rc = gemm8(xf, m->x_fs, m->qd(), L.o_f8, L.o_fs, H, u15::kEpiResid, x, nullptr))) return rc;
+    if ((rc = norm8(L.ln_post))) return rc;
+    if ((rc = gemm8(xf, m->x_fs, H, L.gu_f8, L.gu_fs, 2 * I, u15::kEpiSwigluFp8, m->h_f8, m->h_fs)))
+      return rc;
+    return gemm8(m->h_f8, m->h_fs, I, L.down_f8, L.down_fs, H, u15::kEpiResid, x, nullptr);
+  }
   if ((rc = row_parallel(m->attn + (long)r0 * m->qd(), m->qd(), L.o, L.o8, L.o_s))) return rc;
 
   // ---- MLP half (src/u15-backbone.cc:246-256) ----
@@ -661,6 +725,8 @@ int u15c_model_create_tp(const u15c_config* full, unsigned flags, int tp_rank, i
   if (full->heads % tp_size || full->kv_heads % tp_size || full->inter % (128 * tp_size))
     return fail(U15C_EINVAL, "tensor parallelism: heads and kv_heads must divide by tp_size "
                              "and inter by 128 * tp_size");
+  if (tp_size > 1 && (flags & U15C_MODEL_FP8))
+    return fail(U15C_EINVAL, "tensor parallelism: the fp8 projections run on one device");
   if (u15::dev() == nullptr) return U15C_ECUDA;
   auto* m = new u15c_model();
   m->full = *full;
@@ -695,6 +761,20 @@ int u15c_model_create_tp(const u15c_config* full, unsigned flags, int tp_rank, i
       rc |= m->alloc(&L.gu_s, E * 2 * I * 4, m->allocs);
       rc |= m->alloc(&L.down_s, E * H * 4, m->allocs);
       m->weight_bytes += E * (QKV * H + H * QD + 2 * I * H + H * I) + E * (QKV + 2 * H + 2 * I) * 4;
+    }
+    if (flags & U15C_MODEL_FP8) {
+      // each expert's packed scales apart
+      const size_t sq = E * u15::fp8_scale_bytes(QKV, H), so = E * u15::fp8_scale_bytes(H, QD),
+                   sg = E * u15::fp8_scale_bytes(2 * I, H), sd = E * u15::fp8_scale_bytes(H, I);
+      rc |= m->alloc(&L.qkv_f8, E * QKV * H, m->allocs);
+      rc |= m->alloc(&L.o_f8, E * H * QD, m->allocs);
+      rc |= m->alloc(&L.gu_f8, E * 2 * I * H, m->allocs);
+      rc |= m->alloc(&L.down_f8, E * H * I, m->allocs);
+      rc |= m->alloc(&L.qkv_fs, sq, m->allocs);
+      rc |= m->alloc(&L.o_fs, so, m->allocs);
+      rc |= m->alloc(&L.gu_fs, sg, m->allocs);
+      rc |= m->alloc(&L.down_fs, sd, m->allocs);
+      m->weight_bytes += E * (QKV * H + H * QD + 2 * I * H + H * I) + sq + so + sg + sd;
     }
     if (rc) break;
   }
@@ -985,13 +1065,21 @@ int u15c_model_bind_random(u15c_model* m, u15c_stream stream, uint64_t seed, flo
 int u15c_model_finalize(u15c_model* m, u15c_stream stream)
 {
   if (m == nullptr) return fail(U15C_EINVAL, "null model");
-  if (!(m->flags & U15C_MODEL_INT8)) return U15C_OK;
+  if (!(m->flags & (U15C_MODEL_INT8 | U15C_MODEL_FP8))) return U15C_OK;
   DeviceScope ds(m->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const u15c_config& c = m->cfg;
   const int E = c.n_experts, H = c.hidden, I = c.inter, QD = m->qd(), QKV = m->qkv_n();
   for (auto& L : m->layers) {
     int rc = 0;
+    if (m->flags & U15C_MODEL_FP8) {
+      rc |= u15::launch_quant_weight_fp8(L.qkv, L.qkv_f8, L.qkv_fs, E, QKV, H, st);
+      rc |= u15::launch_quant_weight_fp8(L.o, L.o_f8, L.o_fs, E, H, QD, st);
+      rc |= u15::launch_quant_weight_fp8(L.gu, L.gu_f8, L.gu_fs, E, 2 * I, H, st);
+      rc |= u15::launch_quant_weight_fp8(L.down, L.down_f8, L.down_fs, E, H, I, st);
+      if (rc) return fail(U15C_ECUDA, "finalize: fp8 quantisation launch failed");
+    }
+    if (!(m->flags & U15C_MODEL_INT8)) continue;
     rc |= u15::launch_quant_rows(L.qkv, L.qkv8, L.qkv_s, E * QKV, H, st);
     rc |= u15::launch_quant_rows(L.o, L.o8, L.o_s, E * H, QD, st);
     rc |= u15::launch_quant_rows(L.gu, L.gu8, L.gu_s, E * 2 * I, H, st);
@@ -1008,7 +1096,10 @@ size_t u15c_model_scratch_bytes(const u15c_model* m, int n)
   if (m == nullptr || n <= 0) return 0;
   const size_t H = m->cfg.hidden, I = m->cfg.inter, QD = m->qd(), QKV = m->qkv_n();
   const size_t maxk = std::max({H, I, QD});
-  return (size_t)n * (2 * (H + QKV + 2 * QD + I + H) + 8 * 128 + maxk + 4);
+  size_t fp8 = 0;   // the scales of the activations, the quantised SwiGLU rows
+  if (m->flags & U15C_MODEL_FP8)
+    fp8 = u15::fp8_scale_bytes(n, (int)maxk) + n * I + u15::fp8_scale_bytes(n, (int)I);
+  return (size_t)n * (2 * (H + QKV + 2 * QD + I + H) + 8 * 128 + maxk + 4) + fp8;
 }
 
 size_t u15c_model_kv_bytes(const u15c_model* m, int capacity)

@@ -20,8 +20,8 @@ EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_STORE_F32 = 0, 1, 2, 3
 TP_BLOB_BYTES = 128
 ATTN_BIDIRECTIONAL, ATTN_CAUSAL, ATTN_BLOCK_CAUSAL = 0, 1, 2
 EXPERT_UND, EXPERT_GEN = 0, 1
-MODEL_INT8 = 1
-FWD_INT8, FWD_SAGE = 1, 2
+MODEL_INT8, MODEL_FP8 = 1, 2
+FWD_INT8, FWD_SAGE, FWD_FP8 = 1, 2, 4
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 CFG_NONE, CFG_IMG, CFG_UNC, CFG_BOTH = 0, 1, 2, 3
 NORM_NONE, NORM_GLOBAL, NORM_CHANNEL, NORM_ZERO_STAR = 0, 1, 2, 3

@@ -382,7 +382,7 @@ class Generator:
                  form: int = None, i_img: int = -1, i_unc: int = -1,
                  cfg_interval=(0.0, 1.0), int8: bool = False, sage: bool = False,
                  init_noise: torch.Tensor = None, init_noise_path: str = None,
-                 step_callback=None, noise_scale_max: float = 16.0):
+                 step_callback=None, noise_scale_max: float = 16.0, fp8: bool = False):
         """Run the loop; returns the final [H][W][3] f32 image (device).
         `branches` are already ordered cond, [img_cond], [uncond]. The start
         image is the reference's seeded draw scaled by the resolution's noise
@@ -453,7 +453,7 @@ class Generator:
                     slots.append({"kv": b.kv, "kv_off": npre, "kv_len": npre + Ltok,
                                   "pos": b.pos})
                 self.m.forward_many(hstate[:len(run)], Ltok, slots, expert=L.EXPERT_GEN,
-                                    int8=int8, sage=sage)
+                                    int8=int8, sage=sage, fp8=fp8)
                 for i, bi in enumerate(run):
                     b = branches[bi]
                     self.m.final_norm(hstate[i], L.EXPERT_GEN)

@@ -16,21 +16,26 @@ FULL = dict(n_layers=42, hidden=4096, heads=32, kv_heads=8, head_dim=128, inter=
             n_experts=2, eps=1e-6, theta_t=5e6, theta_hw=1e4)
 
 
+def _fwd_flags(int8, sage, fp8):
+    return (L.FWD_INT8 if int8 else 0) | (L.FWD_SAGE if sage else 0) | (L.FWD_FP8 if fp8 else 0)
+
+
 class Model:
     """U15Weights + U15Backbone for one device, or this rank's share of a
     tensor-parallel model (tp_size > 1: bind full tensors, then install the
     all-reduce with set_allreduce before the first pass)."""
 
-    def __init__(self, int8: bool = False, tp_rank: int = 0, tp_size: int = 1, **cfg):
+    def __init__(self, int8: bool = False, tp_rank: int = 0, tp_size: int = 1, fp8: bool = False,
+                 **cfg):
         c = dict(FULL)
         c.update(cfg)
         self.cfg = c
         self._cfg = L.Config(**c)
         h = C.c_void_p()
-        check(lib().u15c_model_create_tp(C.byref(self._cfg), L.MODEL_INT8 if int8 else 0,
-                                         tp_rank, tp_size, C.byref(h)))
+        flags = (L.MODEL_INT8 if int8 else 0) | (L.MODEL_FP8 if fp8 else 0)
+        check(lib().u15c_model_create_tp(C.byref(self._cfg), flags, tp_rank, tp_size, C.byref(h)))
         self.h = h
-        self.int8 = int8
+        self.int8, self.fp8 = int8, fp8
         self.tp_rank, self.tp_size = tp_rank, tp_size
         self._ar_cb = None
         self._part = None
@@ -130,26 +135,26 @@ class Model:
 
     # ---- backbone -----------------------------------------------------
     def layer_forward(self, layer, x, kv, kv_off, kv_len, pos_t, pos_h, pos_w, segments=None,
-                      attn=L.ATTN_BIDIRECTIONAL, t_index=None, int8=False, sage=False):
+                      attn=L.ATTN_BIDIRECTIONAL, t_index=None, int8=False, sage=False, fp8=False):
         n = x.shape[0]
         off, ex, ns = segments_arrays(segments, n)
-        flags = (L.FWD_INT8 if int8 else 0) | (L.FWD_SAGE if sage else 0)
+        flags = _fwd_flags(int8, sage, fp8)
         check(lib().u15c_layer_forward(self.h, _stream(), layer, _p(x), n, off, ex, ns, kv.h,
                                        kv_off, kv_len, _p(pos_t), _p(pos_h), _p(pos_w), attn,
                                        _p(t_index), flags))
 
     def forward(self, x, kv, kv_off, kv_len, pos_t, pos_h, pos_w, segments=None,
-                attn=L.ATTN_BIDIRECTIONAL, t_index=None, int8=False, sage=False, stop=None):
+                attn=L.ATTN_BIDIRECTIONAL, t_index=None, int8=False, sage=False, stop=None, fp8=False):
         n = x.shape[0]
         off, ex, ns = segments_arrays(segments, n)
-        flags = (L.FWD_INT8 if int8 else 0) | (L.FWD_SAGE if sage else 0)
+        flags = _fwd_flags(int8, sage, fp8)
         cb = L.STOP_FN(lambda _ctx: int(bool(stop()))) if stop is not None else L.STOP_FN()
         check(lib().u15c_forward(self.h, _stream(), _p(x), n, off, ex, ns, kv.h, kv_off, kv_len,
                                  _p(pos_t), _p(pos_h), _p(pos_w), attn, _p(t_index), flags, cb,
                                  None))
 
     def forward_many(self, x, n, slots, expert=L.EXPERT_GEN, attn=L.ATTN_BIDIRECTIONAL,
-                     int8=False, sage=False, stop=None):
+                     int8=False, sage=False, stop=None, fp8=False):
         """x [len(slots) * n][hidden]; slots: list of dicts with kv, kv_off, kv_len,
         pos (t, h, w device int32 tensors) and optional t_index."""
         arr = (L.Slot * len(slots))()
@@ -158,7 +163,7 @@ class Model:
             arr[i] = L.Slot(s["kv"].h, s["kv_off"], s["kv_len"], pt.data_ptr(), ph.data_ptr(),
                             pw.data_ptr(), s["t_index"].data_ptr() if s.get("t_index") is not None
                             else None)
-        flags = (L.FWD_INT8 if int8 else 0) | (L.FWD_SAGE if sage else 0)
+        flags = _fwd_flags(int8, sage, fp8)
         cb = L.STOP_FN(lambda _ctx: int(bool(stop()))) if stop is not None else L.STOP_FN()
         check(lib().u15c_forward_many(self.h, _stream(), _p(x), n, arr, len(slots), expert, attn,
                                       flags, cb, None))
@@ -168,23 +173,23 @@ class Model:
 
     def layer_forward_host(self, layer, x_host, out_host, kv, kv_off, kv_len, pos_t, pos_h,
                            pos_w, segments=None, attn=L.ATTN_BIDIRECTIONAL, t_index=None,
-                           int8=False, sage=False):
+                           int8=False, sage=False, fp8=False):
         n = x_host.shape[0]
         off, ex, ns = segments_arrays(segments, n)
-        flags = (L.FWD_INT8 if int8 else 0) | (L.FWD_SAGE if sage else 0)
+        flags = _fwd_flags(int8, sage, fp8)
         check(lib().u15c_layer_forward_host(self.h, _stream(), layer, _p(x_host), _p(out_host),
                                             n, off, ex, ns, kv.h, kv_off, kv_len, _p(pos_t),
                                             _p(pos_h), _p(pos_w), attn, _p(t_index), flags))
 
     def layer_forward_host_async(self, layer, x_host, out_host, kv, kv_off, kv_len, pos_t, pos_h,
                                  pos_w, segments=None, attn=L.ATTN_BIDIRECTIONAL, t_index=None,
-                                 int8=False, sage=False):
+                                 int8=False, sage=False, fp8=False):
         """Enqueue the layer through pinned host buffers without waiting
         (u15c_layer_forward_host_async): x_host must stay unchanged and
         out_host unread until host_drain() and a stream synchronisation."""
         n = x_host.shape[0]
         off, ex, ns = segments_arrays(segments, n)
-        flags = (L.FWD_INT8 if int8 else 0) | (L.FWD_SAGE if sage else 0)
+        flags = _fwd_flags(int8, sage, fp8)
         check(lib().u15c_layer_forward_host_async(self.h, _stream(), layer, _p(x_host),
                                                   _p(out_host), n, off, ex, ns, kv.h, kv_off,
                                                   kv_len, _p(pos_t), _p(pos_h), _p(pos_w), attn,
