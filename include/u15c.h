@@ -207,7 +207,8 @@ int u15c_kv_append(u15c_stream stream, const void* in, void* pages, const int32_
  * the smallest exponent for which 448 * 2^(s - 127) reaches the largest
  * magnitude of its block (0 when 2^-118 does), so no finite value saturates;
  * values are rounded to nearest even, once. A value that is not finite
- * becomes the NaN code 0x7F and makes every product with its row NaN.
+ * becomes the NaN code 0x7F and makes every product with its row NaN; the
+ * finite values of a block that holds an Inf become 0.
  * Blocks are 1 x 128 for activations, 128 x 128 for weights (the byte is then
  * the same for the block's 128 rows); the last block of a row or a column
  * may be short. cols must be a multiple of 16.
@@ -216,7 +217,7 @@ int u15c_kv_append(u15c_stream stream, const void* in, void* pages, const int32_
  * G = ceil(cols / 512), the byte of (row r, block b) is at
  *   ((r / 128) * G + b / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4
  * in a buffer of u15c_fp8_scale_bytes(rows, cols). Bytes of rows and blocks
- * that do not exist are neither read nor written. Stacked weights keep each
+ * that do not exist count for nothing and are not written. Stacked weights keep each
  * expert's packed scales apart, one after another. q and scale buffers, and
  * the bf16 tensors here, must be 16-byte aligned (y, resid and bias of the
  * products need only their type's alignment). No reference counterpart: the
@@ -248,7 +249,8 @@ int u15c_mot_add_rms_norm_quant_fp8(u15c_stream stream, const void* x, const voi
 
 /* The routed projection of quantised rows xq [M][K] by quantised weights
  * wq_stack [n_experts][N][K]; segments as u15c_mot_linear_bf16. Products are
- * exact, sums f32. epilogue: U15C_EPI_STORE (y = bf16(acc (+ bias))),
+ * exact, sums f32 (in an order that depends on the sizes and segments alone:
+ * the same call gives the same bits). epilogue: U15C_EPI_STORE (y = bf16(acc (+ bias))),
  * U15C_EPI_RESIDUAL (y = bf16(resid + acc), rounded once; y may be resid),
  * U15C_EPI_SWIGLU (N a multiple of 256, rows interleaved in 128-row blocks
  * [gate | up]: y [M][N/2] = bf16(silu(gate) * up), rounded once),

@@ -52,6 +52,10 @@ def test_quantisers(lib):
     refused(lib.u15c_quant_weight_fp8(None, A, A, A, 2, 4, 40), "multiple of 16")
     refused(lib.u15c_dequant_fp8(None, A, A, A + 2, 1, 4, 128), "unaligned")
     refused(lib.u15c_dequant_fp8(None, A, A, A, 1, 4, 0), "cols")
+    refused(lib.u15c_quant_rows_fp8(None, A, A, A, 1 << 30, 16), "2^30")
+    refused(lib.u15c_quant_rows_fp8(None, A, A, A, 4, 1 << 30), "2^30")
+    refused(lib.u15c_quant_weight_fp8(None, A, A, A, 1, 1 << 24, 16), "range")
+    refused(lib.u15c_dequant_fp8(None, A, A, A, 1, 1 << 30, 16), "range")
 
 
 def norm(lib, x=A, delta=None, w=A, ne=2, off=None, ex=None, ns=0, out=None, q=A, s=A, rows=4,
@@ -66,6 +70,8 @@ def test_norm(lib):
     refused(norm(lib, out=A + 1), "unaligned")
     refused(norm(lib, dim=120), "multiple of 16")
     refused(norm(lib, ne=0), "out of")
+    refused(norm(lib, rows=1 << 30), "out of")
+    refused(norm(lib, dim=1 << 30), "out of")
     refused(norm(lib, off=ints(0, 2, 3), ex=ints(0, 1), ns=2), "cover")
     refused(norm(lib, off=ints(0, 2, 4), ex=ints(0, 2), ns=2), "expert")
 
@@ -86,6 +92,8 @@ def test_linear(lib):
     refused(linear(lib, N=0), "positive")
     refused(linear(lib, M=-1), "not negative")
     refused(linear(lib, ne=40, N=1 << 27), "2^31")
+    for k in ("M", "K", "N"):
+        refused(linear(lib, **{k: 1 << 30}), "2^30")
     for k in ("xq", "sx", "wq", "sw", "y"):
         refused(linear(lib, **{k: None}), "null")
     for k in ("xq", "sx", "wq", "sw"):

@@ -122,6 +122,30 @@ def test_quant_weight_bit_exact(ops, E, N, K):
         assert np.array_equal(host(y)[e], F.values(wq, ws).astype(np.float32))
 
 
+def test_calls_side_by_side(ops):
+    """Several products at once on streams of their own give what they give alone."""
+    cases = [(3, 2048, 1024), (100, 1024, 768), (300, 512, 2048), (512, 2048, 4096)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    made, want = [], []
+    for M, K, N in cases:
+        xq, xs, _ = random_quantised(ops, M, K, M, 1.0)
+        wq, ws, _ = random_quantised(ops, N, K, N, 0.05)
+        made.append((xq, xs, wq.view(1, N, K), ws))
+        y = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+        ops.mot_linear_fp8(*made[-1], None, y, M, K, N)
+        want.append(y)
+    torch.cuda.synchronize()
+    out = [torch.empty_like(y) for y in want]
+    for _ in range(10):
+        for st, a, y, (M, K, N) in zip(streams, made, out, cases):
+            with torch.cuda.stream(st):
+                ops.mot_linear_fp8(*a, None, y, M, K, N)
+    torch.cuda.synchronize()
+    ops.sync()
+    for y, t in zip(out, want):
+        assert torch.equal(y, t)
+
+
 def test_scale_buffers_are_sized(ops):
     assert ops.fp8_scale(129, 528, n_experts=2).numel() == 2 * F.scale_bytes(129, 528)
 
@@ -219,6 +243,30 @@ def run_linear(ops, M, K, N, segs, epi, seed=11, bias=False):
 @pytest.mark.parametrize("segs", ["one", "two", "many"])
 def test_linear(ops, M, K, N, segs):
     run_linear(ops, M, K, N, segments_of(M, segs), STORE)
+
+
+def test_linear_empty_and_single_row_segments(ops):
+    """Segments of no rows at either end and in the middle, and of one row."""
+    for M in (3, 70, 150, 600):
+        run_linear(ops, M, 272, 384, [(0, 0, 1), (0, 1, 0), (1, 1, 1), (1, M - 1, 1),
+                                      (M - 1, M, 0), (M, M, 1)], RESID)
+
+
+def test_linear_unaligned_outputs(ops):
+    """y, residual and bias off every 16-byte boundary."""
+    for M, N in [(5, 256), (70, 512), (300, 512)]:
+        K, E = 256, 1
+        xq, xs = quantised(M, K, 15)
+        W, wq, ws = weights(E, N, K, 16)
+        r, b = dev_bf16(randn(M * N + 1, 17))[1:], dev_bf16(randn(N + 1, 18))[1:]
+        args = (dev_u8(xq), dev_u8(F.pack(xs, K)), wq, ws, None)
+        for kw in (dict(epilogue=RESID, resid=r), dict(bias=b)):
+            y = torch.zeros(M * N + 1, dtype=torch.bfloat16, device="cuda")
+            ops.mot_linear_fp8(*args, y[1:], M, K, N, **kw)
+            kw = {k: v.clone() if torch.is_tensor(v) else v for k, v in kw.items()}
+            want = torch.empty(M * N, dtype=torch.bfloat16, device="cuda")
+            ops.mot_linear_fp8(*args, want, M, K, N, **kw)
+            assert torch.equal(y[1:], want) and y[0] == 0
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
@@ -324,7 +372,10 @@ def random_quantised(ops, rows, cols, seed, std):
     (2100, 640, 4096, [(0, 2100, 0)]),                         # a part-empty last round: half-width tiles
     (1800, 512, 6144, [(0, 77, 0), (77, 1800, 1)]),            # several rounds, an odd boundary
     (3000, 384, 2176, [(0, 250, 1), (250, 251, 0), (251, 1600, 1), (1600, 3000, 0)]),
-    (1030, 272, 8192, [(0, 320, 0), (320, 1030, 1)])])
+    (1030, 272, 8192, [(0, 320, 0), (320, 1030, 1)]),
+    # fewer tiles than pairs: two, three and four pairs a tile
+    (512, 2064, 4096, [(0, 512, 0)]), (300, 12288, 2048, [(0, 300, 1)]),
+    (400, 8192, 1536, [(0, 100, 0), (100, 400, 1)]), (450, 2304, 4000, [(0, 130, 1), (130, 450, 0)])])
 @pytest.mark.parametrize("epi", [STORE, RESID, SWIGLU])
 def test_many_tiles(ops, M, K, N, segs, epi):
     """More tiles than CTA pairs: the accumulators' shared columns, the scale
@@ -434,6 +485,10 @@ def test_ffn_is_its_steps(ops, rows, h, i, add):
     rest = (t["w"], t["gu"], t["gs"], t["dn"], t["ds"], segs)
     ops.mot_ffn_fp8(t["x"], t["d"] if add else None, *rest, y, ws, rows, h, i, 1e-6)
     assert torch.equal(t["x"], x0)
+    if add:                                           # over the residual's addend
+        d = t["d"].clone()
+        ops.mot_ffn_fp8(t["x"], d, *rest, d, ws, rows, h, i, 1e-6)
+        assert torch.equal(d, want)
     ops.mot_ffn_fp8(t["x"], t["d"] if add else None, *rest, t["x"], ws, rows, h, i, 1e-6)
     ops.sync()
     assert torch.equal(y, want) and torch.equal(t["x"], want)

@@ -272,6 +272,8 @@ bool aligned16(std::initializer_list<const void*> ptrs)
     if (reinterpret_cast<uintptr_t>(p) & 15) return false;
   return true;
 }
+// sizes whose indexes stay inside int with a grid's stride to spare
+constexpr int kFp8Most = 0x3FFFFFFF;
 }  // namespace
 
 int check_gemm_fp8(const GemmFp8Args& a)
@@ -279,6 +281,8 @@ int check_gemm_fp8(const GemmFp8Args& a)
   if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.n_experts <= 0)
     return fail(U15C_EINVAL, "gemm_fp8: N, K and n_experts must be positive, M not negative");
   if (a.K % 16) return fail(U15C_EINVAL, "gemm_fp8: K must be a multiple of 16");
+  if (a.M > kFp8Most || a.N > kFp8Most || a.K > kFp8Most)
+    return fail(U15C_EINVAL, "gemm_fp8: M, N and K must be below 2^30");
   if ((long)a.N * a.n_experts > 0x7FFFFFFFL)
     return fail(U15C_EINVAL, "gemm_fp8: n_experts * N exceeds 2^31 - 1 rows");
   const bool gu = a.epilogue == kEpiSwiglu || a.epilogue == kEpiSwigluFp8;
@@ -546,10 +550,10 @@ int u15c_quant_rows_fp8(u15c_stream stream, const void* x, uint8_t* q, uint8_t* 
                         int cols)
 {
   if (rows == 0 && cols > 0 && cols % 16 == 0) return U15C_OK;
-  if (x == nullptr || q == nullptr || scale == nullptr || rows < 0 || cols <= 0 || cols % 16 ||
-      !aligned16({x, q, scale}))
-    return fail(U15C_EINVAL, "quant_rows_fp8: null or unaligned buffer, negative rows, or cols not "
-                             "a multiple of 16");
+  if (x == nullptr || q == nullptr || scale == nullptr || rows < 0 || rows > kFp8Most ||
+      cols <= 0 || cols % 16 || cols > kFp8Most || !aligned16({x, q, scale}))
+    return fail(U15C_EINVAL, "quant_rows_fp8: null or unaligned buffer, negative rows, cols not a "
+                             "multiple of 16, or 2^30 of either");
   LAUNCH(launch_quant_rows_fp8(x, q, scale, rows, cols, ST(stream)), "quant_rows_fp8");
 }
 
@@ -557,7 +561,7 @@ int u15c_quant_weight_fp8(u15c_stream stream, const void* w, uint8_t* q, uint8_t
                           int n_experts, int N, int K)
 {
   if (w == nullptr || q == nullptr || scale == nullptr || n_experts <= 0 || n_experts > 65535 ||
-      N <= 0 || N > 65535 * 128 || K <= 0 || K % 16 || !aligned16({w, q, scale}))
+      N <= 0 || N > 65535 * 128 || K <= 0 || K % 16 || K > kFp8Most || !aligned16({w, q, scale}))
     return fail(U15C_EINVAL, "quant_weight_fp8: null or unaligned buffer, sizes out of range, or K "
                              "not a multiple of 16");
   LAUNCH(launch_quant_weight_fp8(w, q, scale, n_experts, N, K, ST(stream)), "quant_weight_fp8");
@@ -567,8 +571,9 @@ int u15c_dequant_fp8(u15c_stream stream, const uint8_t* q, const uint8_t* scale,
                      int n_experts, int rows, int cols)
 {
   if (rows == 0 && n_experts > 0 && cols > 0 && cols % 16 == 0) return U15C_OK;
-  if (q == nullptr || scale == nullptr || y == nullptr || n_experts <= 0 || rows < 0 || cols <= 0 ||
-      cols % 16 || !aligned16({q, scale, y}))
+  if (q == nullptr || scale == nullptr || y == nullptr || n_experts <= 0 || n_experts > 65535 ||
+      rows < 0 || rows > kFp8Most || cols <= 0 || cols % 16 || cols > kFp8Most ||
+      !aligned16({q, scale, y}))
     return fail(U15C_EINVAL, "dequant_fp8: null or unaligned buffer, sizes out of range, or cols "
                              "not a multiple of 16");
   LAUNCH(launch_dequant_fp8(q, scale, y, n_experts, rows, cols, ST(stream)), "dequant_fp8");
@@ -580,8 +585,8 @@ int u15c_mot_add_rms_norm_quant_fp8(u15c_stream stream, const void* x, const voi
                                     uint8_t* scale, int rows, int dim, float eps)
 {
   const bool bufs = rows == 0 || (x != nullptr && q != nullptr && scale != nullptr);
-  if (!bufs || w_stack == nullptr || n_experts <= 0 || rows < 0 || dim <= 0 || dim % 16 ||
-      !aligned16({x, delta, w_stack, x_out, q, scale}))
+  if (!bufs || w_stack == nullptr || n_experts <= 0 || rows < 0 || rows > kFp8Most || dim <= 0 ||
+      dim % 16 || dim > kFp8Most || !aligned16({x, delta, w_stack, x_out, q, scale}))
     return fail(U15C_EINVAL, "add_rms_norm_quant_fp8: null or unaligned buffer, sizes out of "
                              "range, or dim not a multiple of 16");
   SegInfo seg;
@@ -674,8 +679,9 @@ int u15c_mot_ffn_fp8(u15c_stream stream, const void* x, const void* delta,
                      int rows, int hidden, int inter, float eps)
 {
   const bool bufs = rows == 0 || (x != nullptr && y != nullptr && ws != nullptr);
-  if (!bufs || w_norm_stack == nullptr || rows < 0 || n_experts <= 0 || hidden <= 0 ||
-      hidden % 16 || inter <= 0 || inter % 128 || inter > 0x3FFFFFFF ||
+  if (!bufs || w_norm_stack == nullptr || rows < 0 || rows > kFp8Most || n_experts <= 0 ||
+      hidden <= 0 || hidden % 16 || hidden > kFp8Most || inter <= 0 || inter % 128 ||
+      inter > kFp8Most / 2 ||
       !aligned16({x, delta, w_norm_stack, y, ws}))
     return fail(U15C_EINVAL, "ffn_fp8: null or unaligned buffer, negative rows, hidden not a "
                              "multiple of 16 or inter of 128");

@@ -31,6 +31,12 @@ using bf16 = __nv_bfloat16;
 // columns, so the accumulators share 32: tile t + 1's MMAs wait until the
 // epilogue has read those 32 columns of tile t (its first step, ~100 cycles),
 // not the whole tile.
+//
+// SPLIT: fewer tiles than pairs. The k-blocks of a tile are split over the
+// pairs of a cluster of 4, 6 or 8 CTAs, a cluster a tile; each CTA leaves its
+// 128 x 256 partial sums in shared memory, over the ring, and finishes its share
+// of the rows from every pair's (in pair order): 512 rows x 4096 x 12288 are
+// 32 tiles, 37 us on 32 pairs.
 // ---------------------------------------------------------------------
 constexpr int kKps = 2;                        // k-blocks per stage
 constexpr int kStg = 3;
@@ -38,6 +44,7 @@ constexpr int kTileBytes = 128 * 128;          // one operand, one k-block, one 
 constexpr int kStageBytes = 2 * kKps * kTileBytes + 2048;   // operands, then the scales
 constexpr int kSmemPair = kStg * kStageBytes + 1024 /*align*/ + 2048 /*amax*/ + 256 /*bars*/;
 constexpr int kThreadsPair = 320;
+constexpr int kMaxPairs = 4;                   // pairs a tile: clusters of 8 CTAs, the portable size
 constexpr int kAccStep = 224;                  // accumulator 1 starts 32 columns early
 constexpr int kSfCol = 480;                    // two sets of 8 + 8 scale columns
 
@@ -49,6 +56,7 @@ struct PairParams {
   int seg_expert[kMaxSeg];
   int unit_start[kMaxSeg + 1];
   int sf_blk_expert;   // scale row blocks of one expert
+  int split;           // SPLIT: pairs a tile
   void* y;
   const bf16* resid;
   const bf16* bias;
@@ -148,7 +156,70 @@ __device__ __forceinline__ void add32(float (&v)[32], const bf16* src, int col0,
   }
 }
 
-template <int EPI>
+// four columns of a row, of which the first n exist; `whole`: all four, and
+// rows are a multiple of four columns
+__device__ __forceinline__ void add4(float (&v)[4], const bf16* src, bool whole, int n)
+{
+  if (whole && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+    const uint2 u = *reinterpret_cast<const uint2*>(src);
+    const float2 a = unpack_bf2(u.x), b = unpack_bf2(u.y);
+    v[0] += a.x; v[1] += a.y; v[2] += b.x; v[3] += b.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) v[i] += bf2f(src[i]);
+  }
+}
+__device__ __forceinline__ void store4(bf16* dst, const float (&v)[4], bool whole, int n)
+{
+  if (whole && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) dst[i] = f2bf(v[i]);
+  }
+}
+__device__ __forceinline__ void store4(float* dst, const float (&v)[4], bool whole, int n)
+{
+  if (whole && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) dst[i] = v[i];
+  }
+}
+
+// Four finished columns of a row, at column `col` of ncols, a warp a run of 128
+// (with SwiGLU applied): the epilogue's other steps and the store. `blk`: the
+// block of 128 outputs of a quantised row.
+template <int EPI, class P>
+__device__ __forceinline__ void finish4(float (&v)[4], const P& p, long row, int blk, int expert,
+                                        int col, int ncols)
+{
+  if constexpr (EPI == kEpiSwigluFp8) {
+    float m = 0.0f;   // never NaN: fmaxf drops them
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = fmaxf(m, fabsf(v[k]));
+    m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+    const uint32_t sb = fp8_scale_byte(m);
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + row * ncols + col) =
+        fp8_codes4(v, fp8_inv_scale(sb, m));
+    if (lane_id() == 0) p.sy[fp8_scale_at(row, blk, fp8_groups(ncols))] = (uint8_t)sb;
+  } else {
+    const long at = row * ncols + col;
+    const bool whole = col + 4 <= ncols && (ncols & 3) == 0;   // four columns, aligned together
+    if (p.bias != nullptr) add4(v, p.bias + (long)expert * p.N + col, whole, ncols - col);
+    if constexpr (EPI == kEpiResid) add4(v, p.resid + at, whole, ncols - col);
+    if constexpr (EPI == kEpiStoreF32)
+      store4(static_cast<float*>(p.y) + at, v, whole, ncols - col);
+    else
+      store4(static_cast<bf16*>(p.y) + at, v, whole, ncols - col);
+  }
+}
+
+template <int EPI, bool SPLIT>
 __global__ void __launch_bounds__(kThreadsPair, 1)
     gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                          const __grid_constant__ CUtensorMap tmB,
@@ -162,20 +233,22 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* amax_sm = reinterpret_cast<float*>(smem + kStg * kStageBytes);   // [2 tiles][2 halves][128]
+  // [2 tiles][2 halves of the columns][128 rows]
+  float* amax_sm = reinterpret_cast<float*>(smem + kStg * kStageBytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStg * kStageBytes + 2048);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStg + 8);
 
   const uint32_t full0 = smem_u32(bars);        // leader: count 2 (one per CTA) + tx
   const uint32_t empty0 = full0 + 8 * kStg;     // each CTA: leader's multicast commit
-  const uint32_t accf0 = empty0 + 8 * kStg;     // each CTA: leader's multicast commit, per accumulator
+  const uint32_t accf0 = empty0 + 8 * kStg;     // each CTA, per accumulator: the same
   const uint32_t accr = accf0 + 16;             // leader: 512 epilogue threads, a phase a tile
   const uint32_t drain = accr + 8;              // each CTA
-  const uint32_t amax0 = drain + 8;             // each CTA: 64 threads a lane quadrant, a phase a tile
+  const uint32_t amax0 = drain + 8;             // each CTA, a lane quadrant: 64 threads
 
   const uint32_t w = warp_id();
-  const uint32_t rank = cluster_ctarank();
+  const uint32_t cta = cluster_ctarank(), rank = cta & 1, lead_cta = cta & ~1u;   // rank in the pair
   const bool leader = rank == 0;
+  const uint16_t both = (uint16_t)(3u << lead_cta);   // the pair's CTAs, for commits
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStg; ++s) {
       mbar_init(full0 + 8 * s, 2);
@@ -206,7 +279,12 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
   griddep_wait();
 
   const int n_tiles = p.n_full + 2 * (p.n_units * p.n_nblk - p.n_full);
-  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  // tiles of this pair, and the k-blocks of them that it takes
+  const int pair = SPLIT ? blockIdx.x / (2 * p.split) : blockIdx.x >> 1;
+  const int n_pairs = SPLIT ? n_tiles : gridDim.x >> 1;
+  const int n_st = (p.n_kblk + kKps - 1) / kKps, part = SPLIT ? (int)(cta >> 1) : 0;
+  const int kb0 = SPLIT ? part * n_st / p.split * kKps : 0;
+  const int kb1 = SPLIT ? min((part + 1) * n_st / p.split * kKps, p.n_kblk) : p.n_kblk;
   const uint32_t base = smem_u32(smem);
 
   if (w == 0) {
@@ -223,17 +301,17 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
       const uint32_t tx = kTileBytes + (half ? kTileBytes / 2 : kTileBytes);
       const uint32_t tx_sf = half ? 3 * kFp8SfTile : 4 * kFp8SfTile;
       const CUtensorMap *mb = half ? &tmBh : &tmB, *msb = half ? &tmSBh : &tmSB;
-      for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
+      for (int kb = kb0; kb < kb1; kb += kKps, ++it) {
         const uint32_t s = it % kStg, ph = (it / kStg) & 1;
         if (!warp_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) {
           ok = false;
           break;
         }
-        const int nk = min(kKps, p.n_kblk - kb);
-        const uint32_t fb = mapa_shared(full0 + 8 * s, 0);
+        const int nk = min(kKps, kb1 - kb);
+        const uint32_t fb = mapa_shared(full0 + 8 * s, lead_cta);
         const uint32_t st = base + s * kStageBytes;
         // a scale tile serves four k-blocks: it comes with the first of them
-        const bool sfs = (kb & 3) == 0;
+        const bool sfs = kb == kb0 || (kb & 3) == 0;
         if (elect_one()) {
           mbar_arrive_expect_tx_cluster(fb, nk * tx + (sfs ? tx_sf : 0));
           if (sfs) {
@@ -277,20 +355,21 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (lt & 1) * kAccStep;
         const uint32_t a_col = (pair_tile(p, t).m0 >> 5) & 3;   // of the unit's first row: 0 or 2
-        for (int kb = 0; kb < p.n_kblk; kb += kKps, ++it) {
+        for (int kb = kb0; kb < kb1; kb += kKps, ++it) {
           const uint32_t s = it % kStg, ph = (it / kStg) & 1;
           if (!warp_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int nk = min(kKps, p.n_kblk - kb);
+          const int nk = min(kKps, kb1 - kb);
           const uint32_t st = base + s * kStageBytes;
-          if ((kb & 3) == 0) sf_set ^= 1;
+          const bool sfs = kb == kb0 || (kb & 3) == 0;
+          sf_set ^= sfs;
           const uint32_t sfa = tmem_base + kSfCol + sf_set * 16, sfb = sfa + 8;
           const uint64_t ad = smem_desc_sw128(st), bd = smem_desc_sw128(st + kKps * kTileBytes);
           if (elect_one()) {
-            if ((kb & 3) == 0) {
+            if (sfs) {
               const uint64_t sf = smem_desc_sf(st + 2 * kKps * kTileBytes);
               sf_copy_pair(sfa, sf);
               if (a_col) sf_copy_pair(sfa + 4, sf + (kFp8SfTile >> 4));
@@ -306,25 +385,25 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
               for (int k = 0; k < 4; ++k)
                 mma_e4m3_pair(d_tmem, ad + hk * (kTileBytes >> 4) + k * 2,
                               bd + hk * (kTileBytes >> 4) + k * 2, id, sfa + a_col, sfb,
-                              ((kb + hk) | k) != 0);
+                              ((kb - kb0 + hk) | k) != 0);
             }
-            mma_commit_pair_mc(empty0 + 8 * s, 0x3);
+            mma_commit_pair_mc(empty0 + 8 * s, both);
           }
           __syncwarp();
         }
-        if (ok && elect_one()) mma_commit_pair_mc(accf0 + 8 * (lt & 1), 0x3);
+        if (ok && elect_one()) mma_commit_pair_mc(accf0 + 8 * (lt & 1), both);
         __syncwarp();
       }
-      if (elect_one()) mma_commit_pair_mc(drain, 0x3);
+      if (elect_one()) mma_commit_pair_mc(drain, both);
       __syncwarp();
     }
     // both CTAs: every MMA that writes this CTA's TMEM has completed
     warp_wait(drain, 0, p.err, kDevWaitDrain);
-  } else {
+  } else if constexpr (!SPLIT) {
     // ---------------- epilogue (warps 2..9, both CTAs) ----------------
     const int wq = (int)(w & 3), wh = (int)(w - 2) >> 2;   // lane quadrant, half of the columns
     const int r_in = wq * 32 + (int)lane_id();
-    const uint32_t accr_leader = mapa_shared(accr, 0);
+    const uint32_t accr_leader = mapa_shared(accr, lead_cta);
     int lt = 0;
     for (int t = pair; t < n_tiles; t += n_pairs, ++lt) {
       const PairTile ti = pair_tile(p, t);
@@ -398,7 +477,8 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
                 for (int j = 0; j < 8; ++j) v[j] = h[i][q * 8 + j];
                 c[q] = fp8_codes8(v, inv);
               }
-              const uint32_t o[8] = {c[0].x, c[0].y, c[1].x, c[1].y, c[2].x, c[2].y, c[3].x, c[3].y};
+              const uint32_t o[8] = {c[0].x, c[0].y, c[1].x, c[1].y,
+                                     c[2].x, c[2].y, c[3].x, c[3].y};
               if (whole_sectors) {
                 store32b(yrow + run[i] * 32, o);
               } else {
@@ -441,9 +521,94 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
     }
   }
 
+  if constexpr (SPLIT) {
+    // ---------------- partial sums, then whole rows ----------------
+    // row r's 16-byte chunk c at r * 1024 + (c ^ (r & 7)) * 16: lanes that hold a row
+    // each write, and a warp that takes a row reads, without bank conflicts
+    const PairTile ti = pair_tile(p, pair);
+    bool ok = true;
+    if (w >= 2) {
+      ok = warp_wait(accf0, 0, p.err, kDevWaitAccFull);
+      tc_fence_after();
+      const int wq = (int)(w & 3), wh = (int)(w - 2) >> 2, r_in = wq * 32 + (int)lane_id();
+#pragma unroll 1
+      for (int c = wh * 4; c < wh * 4 + 4; ++c) {
+        uint32_t v[32];
+        tmem_ld32(tmem_base + ((uint32_t)(wq * 32) << 16) + c * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(smem + r_in * 1024 + (((c * 8 + i) ^ (r_in & 7)) << 4)) =
+              make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      }
+    }
+    __syncthreads();
+    cluster_sync();
+    if (ok) {
+      const int first = ti.m0 + 128 * (int)rank, step = (kThreadsPair / 32) * p.split;
+      const int lo = max(ti.row_lo - first, 0), hi = min(ti.row_hi - first, 128);
+      const int lane = (int)lane_id();
+      // R rows a step of a warp from up to Q pairs, all their loads in flight
+      auto finish = [&](auto r_, auto q_) {
+        constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
+        for (int j0 = lo + part + (int)w * p.split; j0 < hi; j0 += R * step) {
+          float4 v[Q][R][2] = {};
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            if (q >= p.split) break;
+            const uint32_t from = mapa_shared(base, 2 * q + rank);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+              const int j = j0 + i * step;
+              if (j >= hi) break;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                v[q][i][h] = ld_cluster4(from + j * 1024 + (((lane + 32 * h) ^ (j & 7)) << 4));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            if (j0 + i * step >= hi) break;
+            float t[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float4 a = v[0][i][h];
+#pragma unroll
+              for (int q = 1; q < Q; ++q) {
+                a.x += v[q][i][h].x;
+                a.y += v[q][i][h].y;
+                a.z += v[q][i][h].z;
+                a.w += v[q][i][h].w;
+              }
+              t[h][0] = a.x;
+              t[h][1] = a.y;
+              t[h][2] = a.z;
+              t[h][3] = a.w;
+            }
+            const long row = first + j0 + i * step;
+            if constexpr (GU) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) t[0][k] = swiglu1(t[0][k], t[1][k]);
+              finish4<EPI>(t[0], p, row, ti.nb, ti.expert, ti.nb * 128 + lane * 4, p.N / 2);
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                finish4<EPI>(t[h], p, row, ti.nb, ti.expert, ti.nb * 256 + h * 128 + lane * 4, p.N);
+            }
+          }
+        }
+      };
+      using std::integral_constant;
+      if (p.split == 2)
+        finish(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+      else
+        finish(integral_constant<int, 2>{}, integral_constant<int, kMaxPairs>{});
+    }
+  }
+
   tc_fence_before();
   __syncthreads();
-  cluster_sync();   // the peer's smem and TMEM stay alive until the pair is done
+  cluster_sync();   // the peers' smem and TMEM stay alive until all are done
   if (w == 0) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
@@ -502,47 +667,13 @@ struct FewParams {
   unsigned* err;
 };
 
-// four columns of a row, of which the first n exist; `whole`: all four, and
-// rows are a multiple of four columns
-__device__ __forceinline__ void add4(float (&v)[4], const bf16* src, bool whole, int n)
-{
-  if (whole && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
-    const uint2 u = *reinterpret_cast<const uint2*>(src);
-    const float2 a = unpack_bf2(u.x), b = unpack_bf2(u.y);
-    v[0] += a.x; v[1] += a.y; v[2] += b.x; v[3] += b.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) v[i] += bf2f(src[i]);
-  }
-}
-__device__ __forceinline__ void store4(bf16* dst, const float (&v)[4], bool whole, int n)
-{
-  if (whole && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) dst[i] = f2bf(v[i]);
-  }
-}
-__device__ __forceinline__ void store4(float* dst, const float (&v)[4], bool whole, int n)
-{
-  if (whole && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) dst[i] = v[i];
-  }
-}
-
 template <int MT, int EPI>
 __global__ void __launch_bounds__(kThreadsFew, 1)
     gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmX,
                         const __grid_constant__ CUtensorMap tmW,
                         const __grid_constant__ CUtensorMap tmSX,
-                        const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ FewParams p)
+                        const __grid_constant__ CUtensorMap tmSW,
+                        const __grid_constant__ FewParams p)
 {
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   using C = FewCfg<MT, GU>;
@@ -637,8 +768,8 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   if (w == 0) {
     int it = min(C::kStages, n_it);
     for (; it < n_it; ++it) {
-      if (!warp_wait(empty0 + 8 * (it % C::kStages), (it / C::kStages & 1) ^ 1, p.err, kDevWaitEmpty))
-        break;
+      const int s = it % C::kStages, ph = (it / C::kStages) & 1;
+      if (!warp_wait(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) break;
       load(it);
     }
     for (int s = 0; s < C::kStages; ++s)   // every fill has landed before the CTA may exit
@@ -738,7 +869,8 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
           for (int h = 0; h < NA; ++h)
 #pragma unroll
             for (int i = 0; i < R; ++i)
-              if (j0 + i * step < hi) v[q][h][i] = ld_cluster4(from + (h * MT + j0 + i * step) * 512);
+              if (j0 + i * step < hi)
+                v[q][h][i] = ld_cluster4(from + (h * MT + j0 + i * step) * 512);
         }
         float4 t[NA][R];
 #pragma unroll
@@ -764,26 +896,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
             v[2] = swiglu1(v[2], t[1][i].z);
             v[3] = swiglu1(v[3], t[1][i].w);
           }
-          const long row = m0 + j0 + i * step;
-          if constexpr (EPI == kEpiSwigluFp8) {
-            float m = 0.0f;   // never NaN: fmaxf drops them
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m = fmaxf(m, fabsf(v[k]));
-            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-            const uint32_t sb = fp8_scale_byte(m);
-            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + row * ncols + col) =
-                fp8_codes4(v, fp8_inv_scale(sb, m));
-            if (lane_id() == 0) p.sy[fp8_scale_at(row, tile, fp8_groups(ncols))] = (uint8_t)sb;
-          } else {
-            const long at = row * ncols + col;
-            const bool whole = col + 4 <= ncols && (ncols & 3) == 0;   // four columns, aligned together
-            if (p.bias != nullptr) add4(v, p.bias + (long)expert * p.N + col, whole, ncols - col);
-            if constexpr (EPI == kEpiResid) add4(v, p.resid + at, whole, ncols - col);
-            if constexpr (EPI == kEpiStoreF32)
-              store4(static_cast<float*>(p.y) + at, v, whole, ncols - col);
-            else
-              store4(static_cast<bf16*>(p.y) + at, v, whole, ncols - col);
-          }
+          finish4<EPI>(v, p, m0 + j0 + i * step, tile, expert, col, ncols);
         }
       }
     };
@@ -803,13 +916,46 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   }
 }
 
-// Persistent grid: as many pairs as can be resident at once (not every SM has
-// a usable partner).
-template <int EPI>
-int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+// Clusters of 1 to kMaxPairs pairs that can be resident (not every SM has a
+// usable partner, and larger clusters leave more SMs out), asked once per kernel
+// and device; null where the device refuses the kernel.
+template <int EPI, bool SPLIT>
+const int* pair_resident(int num_sms)
 {
   static std::atomic<uint64_t> attr_set;
-  static std::atomic<int> max_pairs_dev[64];   // resident pairs, per device (0: not yet known)
+  static std::mutex mu;
+  static int resident_dev[64][kMaxPairs + 1];
+  auto k = gemm_fp8_pair_kernel<EPI, SPLIT>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || !smem_attr_once(k, kSmemPair, attr_set)) return nullptr;
+  std::lock_guard<std::mutex> g(mu);
+  int* r = resident_dev[dev & 63];
+  if (r[0] != 0) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreadsPair);
+  cfg.dynamicSmemBytes = kSmemPair;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  for (int s = 1; s <= kMaxPairs; ++s) {
+    attr[0].val.clusterDim.x = 2 * s;
+    cfg.gridDim = dim3(2 * s);
+    if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0)
+      r[s] = std::max(1, num_sms / (4 * s));
+  }
+  r[0] = 1;   // the entries are there
+  return r;
+}
+
+// split 1: a persistent grid of as many pairs as can be resident at once; more:
+// that many pairs a tile, a cluster a tile.
+template <int EPI, bool SPLIT>
+int launch_pair(const GemmFp8Args& a, const SegInfo& seg, int split, cudaStream_t st,
+                std::string* err)
+{
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   PairParams p{};
   p.M = a.M;
@@ -833,6 +979,7 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
   p.n_nblk = (a.N + 255) / 256;
   p.n_kblk = fp8_blocks(a.K);
   p.sf_blk_expert = (a.N + 127) / 128;
+  p.split = split;
   if ((long)p.n_units * p.n_nblk > 0x3FFFFFFFL) {
     *err = "gemm_fp8: too many output tiles";
     return 1;
@@ -840,44 +987,46 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
   CUtensorMap ma, mb, mbh, msa, msb, msbh;
   const uint64_t wrows = (uint64_t)a.N * a.n_experts, groups = fp8_groups(a.K),
                  wblks = (uint64_t)p.sf_blk_expert * a.n_experts, xblks = (a.M + 127) / 128;
-  if (make_tma_2d(&ma, a.xq, a.M, a.K, 128, 1, err) || make_tma_2d(&mb, a.wq, wrows, a.K, 128, 1, err) ||
+  if (make_tma_2d(&ma, a.xq, a.M, a.K, 128, 1, err) ||
+      make_tma_2d(&mb, a.wq, wrows, a.K, 128, 1, err) ||
       make_tma_2d(&mbh, a.wq, wrows, a.K, 64, 1, err) ||
       make_tma_fp8_scales(&msa, a.sx, xblks, groups, 2, err) ||
       make_tma_fp8_scales(&msb, a.sw, wblks, groups, 2, err) ||
       make_tma_fp8_scales(&msbh, a.sw, wblks, groups, 1, err))
     return 2;
-  auto k = gemm_fp8_pair_kernel<EPI>;
-  if (!smem_attr_once(k, kSmemPair, attr_set)) return 2;
+  const int* resident = pair_resident<EPI, SPLIT>(a.num_sms);
+  if (resident == nullptr) return 2;
+  const int tiles = p.n_units * p.n_nblk;
+  int ctas;
+  if constexpr (SPLIT) {
+    p.n_full = tiles;
+    ctas = 2 * split * tiles;
+  } else {
+    // a last round that would leave at least half the pairs idle runs as
+    // half-width tiles (a SwiGLU tile holds whole gate and up blocks: it is not
+    // split)
+    const int pairs = std::min(tiles, resident[1]), rest = tiles % pairs;
+    p.n_full = !GU && rest > 0 && 2 * rest <= pairs ? tiles - rest : tiles;
+    ctas = 2 * pairs;
+  }
   cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kThreadsPair);
   cfg.dynamicSmemBytes = kSmemPair;
   cfg.stream = st;
   cudaLaunchAttribute attrs[2] = {};
   attrs[0].id = cudaLaunchAttributeClusterDimension;
-  attrs[0].val.clusterDim.x = 2;
+  attrs[0].val.clusterDim.x = 2 * split;
   attrs[0].val.clusterDim.y = 1;
   attrs[0].val.clusterDim.z = 1;
   attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attrs;
-  cfg.numAttrs = 1;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 2;
-  int max_pairs = max_pairs_dev[dev & 63].load(std::memory_order_relaxed);
-  if (max_pairs <= 0) {
-    cfg.gridDim = dim3(2);
-    if (cudaOccupancyMaxActiveClusters(&max_pairs, k, &cfg) != cudaSuccess || max_pairs <= 0)
-      max_pairs = 64;
-    max_pairs_dev[dev & 63].store(max_pairs, std::memory_order_relaxed);
-  }
-  // a last round that would leave at least half the pairs idle runs as
-  // half-width tiles (a SwiGLU tile holds whole gate and up blocks: it is not
-  // split)
-  const int tiles = p.n_units * p.n_nblk, pairs = std::min(tiles, max_pairs), rest = tiles % pairs;
-  p.n_full = !GU && rest > 0 && 2 * rest <= pairs ? tiles - rest : tiles;
-  cfg.gridDim = dim3(2 * pairs);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k, ma, mb, mbh, msa, msb, msbh, p) == cudaSuccess ? 0 : 2;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel<EPI, SPLIT>, ma, mb, mbh, msa, msb, msbh,
+                            p) == cudaSuccess
+             ? 0
+             : 2;
 }
 
 // Row units of height h over the segments: blocks of h rows of the whole pass
@@ -911,7 +1060,8 @@ inline FewPlan few_plan(long tiles, int n_stages, int stage_ns, int round_ns, co
   FewPlan best;
   for (int s = 1; s <= kMaxSplit && s <= n_stages; ++s) {
     const long rounds = (tiles + resident[s] - 1) / resident[s];
-    const long ns = rounds * ((n_stages + s - 1) / s * (long)stage_ns + round_ns) + (s > 1 ? 400 + 50 * s : 0);
+    const long ns = rounds * ((n_stages + s - 1) / s * (long)stage_ns + round_ns) +
+                    (s > 1 ? 400 + 50 * s : 0);
     if (best.ns < 0 || ns < best.ns) best = FewPlan{s, ns};
   }
   return best;
@@ -950,12 +1100,18 @@ const int* few_resident(int num_sms)
   return r;
 }
 
+template <int EPI>
+int few_tiles(const GemmFp8Args& a)
+{
+  return EPI == kEpiSwiglu || EPI == kEpiSwigluFp8 ? a.N / 256 : (a.N + 127) / 128;
+}
+
 template <int MT, int EPI>
 FewPlan few_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* resident)
 {
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   using C = FewCfg<MT, GU>;
-  const long tiles = (long)(GU ? a.N / 256 : (a.N + 127) / 128) * few_units(seg, MT);
+  const long tiles = (long)few_tiles<EPI>(a) * few_units(seg, MT);
   // a k-block of 128 weight rows: 160 ns, or 400 with 128 activation rows
   // beside them; a round's set-up, first loads and epilogue: 2.5 us and 20 ns a row
   const int stage_ns = C::kKps * C::kNA * (MT <= 64 ? 160 : 400);
@@ -989,7 +1145,7 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cu
   }
   p.seg_off[seg.nseg] = seg.off[seg.nseg];
   p.unit_start[seg.nseg] = units;
-  const int tiles = GU ? a.N / 256 : (a.N + 127) / 128;
+  const int tiles = few_tiles<EPI>(a);
   CUtensorMap mx, mw, msx, msw;
   const uint64_t groups = fp8_groups(a.K);
   if (make_tma_2d(&mx, a.xq, a.M, a.K, MT, 1, err) ||
@@ -1016,33 +1172,56 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cu
              : 2;
 }
 
+// More than 64 rows: tiles of 256 rows (pairs, one or several a tile) or of 128.
+template <int EPI>
+int launch_many(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+{
+  const long n_st = (fp8_blocks(a.K) + kKps - 1) / kKps;
+  const long tiles = (long)pair_units(seg) * ((a.N + 255) / 256);
+  const int* one = pair_resident<EPI, false>(a.num_sms);
+  if (one == nullptr) return 2;
+  // measured: 700 ns a stage of a pair and 5.5 us to start and finish; 850 ns
+  // and 8.5 us where partial sums meet (512 rows x 4096 x 12288: one pair a
+  // tile 37 us, two 29.5, tiles of 128 rows 40; 256 rows: 37, three pairs 23.5,
+  // tiles of 128 rows 22.6; 256 x 24576 x 4096 SwiGLU: 30 and 57)
+  int split = 1;
+  long pair_ns = (tiles + one[1] - 1) / one[1] * n_st * 700 + 5500;
+  if (tiles < one[1]) {
+    const int* more = pair_resident<EPI, true>(a.num_sms);
+    if (more == nullptr) return 2;
+    for (int s = 2; s <= kMaxPairs && s <= n_st; ++s) {
+      const long ns = (tiles + more[s] - 1) / more[s] * ((n_st + s - 1) / s * 850 + 8500);
+      if (ns < pair_ns) {
+        pair_ns = ns;
+        split = s;
+      }
+    }
+  }
+  if (a.M <= kFewRows && few_tiles<EPI>(a) <= 65535) {
+    const int* resident = few_resident<128, EPI>(a.num_sms);
+    if (resident == nullptr) return 2;
+    const FewPlan few = few_plan_of<128, EPI>(a, seg, resident);
+    if (few.ns < pair_ns) return launch_few<128, EPI>(a, seg, few, st, err);
+  }
+  return split > 1 ? launch_pair<EPI, true>(a, seg, split, st, err)
+                   : launch_pair<EPI, false>(a, seg, 1, st, err);
+}
+
 template <int MT, int EPI>
-int launch_few_or_pair(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
+int launch_few_rows(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
 {
   const int* resident = few_resident<MT, EPI>(a.num_sms);
   if (resident == nullptr) return 2;
-  const FewPlan few = few_plan_of<MT, EPI>(a, seg, resident);
-  if (MT == 128) {
-    // 256 rows a tile against 128: the pairs' time is their rounds times 700 ns
-    // a stage (512 x 4096 x 12288: pairs 38 us, this form 40; 256 rows: 37 and
-    // 23; 256 x 24576 x 4096 SwiGLU: 30 and 57)
-    const long tiles = (long)pair_units(seg) * ((a.N + 255) / 256);
-    const long rounds = (tiles + a.num_sms / 2 - 1) / (a.num_sms / 2);
-    const long pair_ns = rounds * ((fp8_blocks(a.K) + kKps - 1) / kKps) * 700 + 5500;
-    if (pair_ns <= few.ns) return launch_pair<EPI>(a, seg, st, err);
-  }
-  return launch_few<MT, EPI>(a, seg, few, st, err);
+  return launch_few<MT, EPI>(a, seg, few_plan_of<MT, EPI>(a, seg, resident), st, err);
 }
 
 template <int EPI>
 int launch_rows(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
 {
-  const int tiles = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8 ? a.N / 256 : (a.N + 127) / 128;
-  if (a.M > kFewRows || tiles > 65535) return launch_pair<EPI>(a, seg, st, err);
-  if (a.M <= 16) return launch_few_or_pair<16, EPI>(a, seg, st, err);
-  if (a.M <= 32) return launch_few_or_pair<32, EPI>(a, seg, st, err);
-  if (a.M <= 64) return launch_few_or_pair<64, EPI>(a, seg, st, err);
-  return launch_few_or_pair<128, EPI>(a, seg, st, err);
+  if (a.M > 64 || few_tiles<EPI>(a) > 65535) return launch_many<EPI>(a, seg, st, err);
+  if (a.M <= 16) return launch_few_rows<16, EPI>(a, seg, st, err);
+  if (a.M <= 32) return launch_few_rows<32, EPI>(a, seg, st, err);
+  return launch_few_rows<64, EPI>(a, seg, st, err);
 }
 
 }  // namespace
