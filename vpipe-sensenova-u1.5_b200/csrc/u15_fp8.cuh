@@ -249,6 +249,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
         "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
+// Meet the cluster without ordering memory: for CTAs that have read their peers'
+// shared memory (the loads' values are there) and may then exit. The releasing
+// form waits for the results' global stores first.
+__device__ __forceinline__ void cluster_sync_relaxed()
+{
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // 16 bytes of another CTA of the cluster's shared memory
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr)
 {

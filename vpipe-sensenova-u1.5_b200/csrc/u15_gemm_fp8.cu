@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
       // the 32 columns the accumulators share are the last of accumulator 0
       // and the first of accumulator 1; their warps read them first
       const bool shared_here = wh == (acc ^ 1);
-      bool released = false;
+      bool released = t + n_pairs >= n_tiles;   // nobody waits for the last tile's
       auto release = [&] {
         if (released) return;
         released = true;
@@ -608,7 +608,10 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync();   // the peers' smem and TMEM stay alive until all are done
+  // The peers' shared memory and TMEM stay alive until all are done with them:
+  // every arrival on the leader's barriers and every commit has been waited for,
+  // and partial sums are read, so nothing needs the results' stores to land first
+  cluster_sync_relaxed();
   if (w == 0) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
@@ -909,7 +912,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync();   // the peers have read this CTA's partial sums
+  cluster_sync_relaxed();   // the peers have read this CTA's partial sums
   if (w == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kCols);
