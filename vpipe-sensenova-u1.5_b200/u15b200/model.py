@@ -144,7 +144,8 @@ class Model:
                                        _p(t_index), flags))
 
     def forward(self, x, kv, kv_off, kv_len, pos_t, pos_h, pos_w, segments=None,
-                attn=L.ATTN_BIDIRECTIONAL, t_index=None, int8=False, sage=False, stop=None, fp8=False):
+                attn=L.ATTN_BIDIRECTIONAL, t_index=None, int8=False, sage=False, stop=None,
+                fp8=False):
         n = x.shape[0]
         off, ex, ns = segments_arrays(segments, n)
         flags = _fwd_flags(int8, sage, fp8)

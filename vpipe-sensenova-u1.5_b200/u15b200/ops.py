@@ -25,10 +25,15 @@ def _p(t):
 def _stream():
     # the raw handle: 0.2 us, where building torch.cuda.current_stream() took 3.3 us,
     # as long as the launch itself
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return _raw_stream(torch.cuda.current_device())
 
 
-_INTS = [C.c_int * n for n in range(10)]   # array types, kept: making one takes longer than filling it
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice   # the current device, for calls that hold CUDA tensors
+
+
+# array types, kept: making one takes longer than filling it
+_INTS = [C.c_int * n for n in range(10)]
 
 
 def segments_arrays(segments, rows):
@@ -170,30 +175,30 @@ class CudaOps:
                      torch.uint8)
 
     def quant_rows_fp8(self, x, q, scale, rows, cols):
-        n, d = rows * cols, torch.cuda.current_device()
-        check(lib().u15c_quant_rows_fp8(_stream(), _need(d, "x", x, n, _BF16),
+        n, d = rows * cols, _device()
+        check(lib().u15c_quant_rows_fp8(_raw_stream(d), _need(d, "x", x, n, _BF16),
                                         _need(d, "q", q, n, _E4M3),
                                         _need_scale(d, "scale", scale, rows, cols), rows, cols))
 
     def quant_weight_fp8(self, w, q, scale, n_experts, N, K):
-        n, d = n_experts * N * K, torch.cuda.current_device()
-        check(lib().u15c_quant_weight_fp8(_stream(), _need(d, "w", w, n, _BF16),
+        n, d = n_experts * N * K, _device()
+        check(lib().u15c_quant_weight_fp8(_raw_stream(d), _need(d, "w", w, n, _BF16),
                                           _need(d, "q", q, n, _E4M3),
                                           _need_scale(d, "scale", scale, N, K, n_experts),
                                           n_experts, N, K))
 
     def dequant_fp8(self, q, scale, y, rows, cols, n_experts=1):
-        n, d = n_experts * rows * cols, torch.cuda.current_device()
-        check(lib().u15c_dequant_fp8(_stream(), _need(d, "q", q, n, _E4M3),
+        n, d = n_experts * rows * cols, _device()
+        check(lib().u15c_dequant_fp8(_raw_stream(d), _need(d, "q", q, n, _E4M3),
                                      _need_scale(d, "scale", scale, rows, cols, n_experts),
                                      _need(d, "y", y, n, _BF16), n_experts, rows, cols))
 
     def mot_add_rms_norm_quant_fp8(self, x, delta, w_stack, segments, x_out, q, scale, rows, dim,
                                    eps):
         off, ex, ns = segments_arrays(segments, rows)
-        n, d, E = rows * dim, torch.cuda.current_device(), w_stack.shape[0]
+        n, d, E = rows * dim, _device(), w_stack.shape[0]
         check(lib().u15c_mot_add_rms_norm_quant_fp8(
-            _stream(), _need(d, "x", x, n, _BF16),
+            _raw_stream(d), _need(d, "x", x, n, _BF16),
             None if delta is None else _need(d, "delta", delta, n, _BF16),
             _need(d, "w_stack", w_stack, E * dim, _BF16), E, off, ex, ns,
             None if x_out is None else _need(d, "x_out", x_out, n, _BF16),
@@ -203,10 +208,10 @@ class CudaOps:
     def mot_linear_fp8(self, xq, sx, wq_stack, sw_stack, segments, y, M, K, N,
                        epilogue=L.EPI_STORE, resid=None, bias=None):
         off, ex, ns = segments_arrays(segments, M)
-        d, E = torch.cuda.current_device(), wq_stack.shape[0]
+        d, E = _device(), wq_stack.shape[0]
         ny = M * (N // 2 if epilogue == L.EPI_SWIGLU else N)
         check(lib().u15c_mot_linear_fp8(
-            _stream(), _need(d, "xq", xq, M * K, _E4M3), _need_scale(d, "sx", sx, M, K),
+            _raw_stream(d), _need(d, "xq", xq, M * K, _E4M3), _need_scale(d, "sx", sx, M, K),
             _need(d, "wq_stack", wq_stack, E * N * K, _E4M3),
             _need_scale(d, "sw_stack", sw_stack, N, K, E), E, off, ex, ns, epilogue,
             None if bias is None else _need(d, "bias", bias, E * N, _BF16),
@@ -215,9 +220,9 @@ class CudaOps:
 
     def mot_swiglu_fp8(self, xq, sx, wq_stack, sw_stack, segments, yq, sy, M, K, N):
         off, ex, ns = segments_arrays(segments, M)
-        d, E = torch.cuda.current_device(), wq_stack.shape[0]
+        d, E = _device(), wq_stack.shape[0]
         check(lib().u15c_mot_swiglu_fp8(
-            _stream(), _need(d, "xq", xq, M * K, _E4M3), _need_scale(d, "sx", sx, M, K),
+            _raw_stream(d), _need(d, "xq", xq, M * K, _E4M3), _need_scale(d, "sx", sx, M, K),
             _need(d, "wq_stack", wq_stack, E * N * K, _E4M3),
             _need_scale(d, "sw_stack", sw_stack, N, K, E), E, off, ex, ns,
             _need(d, "yq", yq, M * (N // 2), _E4M3), _need_scale(d, "sy", sy, M, N // 2), M, K,
@@ -230,10 +235,10 @@ class CudaOps:
     def mot_ffn_fp8(self, x, delta, w_norm_stack, gu, gu_scale, down, down_scale, segments, y, ws,
                     rows, hidden, inter, eps):
         off, ex, ns = segments_arrays(segments, rows)
-        d, E, n = torch.cuda.current_device(), gu.shape[0], rows * hidden
+        d, E, n = _device(), gu.shape[0], rows * hidden
         ws_n = lib().u15c_ffn_fp8_workspace_bytes(rows, hidden, inter)
         check(lib().u15c_mot_ffn_fp8(
-            _stream(), _need(d, "x", x, n, _BF16),
+            _raw_stream(d), _need(d, "x", x, n, _BF16),
             None if delta is None else _need(d, "delta", delta, n, _BF16),
             _need(d, "w_norm_stack", w_norm_stack, E * hidden, _BF16),
             _need(d, "gu", gu, E * 2 * inter * hidden, _E4M3),
