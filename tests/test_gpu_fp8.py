@@ -162,7 +162,8 @@ def check_normed(q, s, y, rows, dim):
 
 
 @pytest.mark.parametrize("rows,dim", [(1, 16), (1, 4096), (7, 128), (130, 1040), (33, 4096),
-                                      (65, 4112), (9, 12288)])
+                                      (65, 4112), (9, 12288), (3, 16400), (5000, 272),
+                                      (1200, 4096)])
 @pytest.mark.parametrize("form", ["plain", "add", "add_in_place", "add_unstored", "copy"])
 def test_norm(ops, rows, dim, form):
     x = activations(rows, dim, 1)

@@ -49,7 +49,7 @@ constexpr int kAccStep = 224;                  // accumulator 1 starts 32 column
 constexpr int kSfCol = 480;                    // two sets of 8 + 8 scale columns
 
 struct PairParams {
-  int M, N, K;
+  int N;
   int n_units, n_nblk, n_kblk, n_full;
   int nseg;
   int seg_off[kMaxSeg + 1];
@@ -657,7 +657,7 @@ struct FewCfg {
 };
 
 struct FewParams {
-  int M, N, n_kblk;
+  int N, n_kblk;
   int nseg;
   int seg_off[kMaxSeg + 1];
   int seg_expert[kMaxSeg];
@@ -919,6 +919,19 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   }
 }
 
+// Row units of segment s: blocks of h rows of the whole pass, cut at the segment's
+// ends, or (pairs) blocks of 256 from its first row rounded down to 64.
+inline int few_units_of(const SegInfo& seg, int s, int h)
+{
+  const int lo = seg.off[s], hi = seg.off[s + 1];
+  return hi > lo ? (hi + h - 1) / h - lo / h : 0;
+}
+inline int pair_units_of(const SegInfo& seg, int s)
+{
+  const int lo = seg.off[s], hi = seg.off[s + 1];
+  return hi > lo ? (hi - (lo & ~63) + 255) / 256 : 0;
+}
+
 // Clusters of 1 to kMaxPairs pairs that can be resident (not every SM has a
 // usable partner, and larger clusters leave more SMs out), asked once per kernel
 // and device; null where the device refuses the kernel.
@@ -946,8 +959,10 @@ const int* pair_resident(int num_sms)
   for (int s = 1; s <= kMaxPairs; ++s) {
     attr[0].val.clusterDim.x = 2 * s;
     cfg.gridDim = dim3(2 * s);
-    if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0)
+    if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0) {
+      cudaGetLastError();   // an estimate serves
       r[s] = std::max(1, num_sms / (4 * s));
+    }
   }
   r[0] = 1;   // the entries are there
   return r;
@@ -961,9 +976,7 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, int split, cudaStream_
 {
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   PairParams p{};
-  p.M = a.M;
   p.N = a.N;
-  p.K = a.K;
   p.y = a.y;
   p.resid = static_cast<const bf16*>(a.resid);
   p.bias = static_cast<const bf16*>(a.bias);
@@ -974,8 +987,7 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, int split, cudaStream_
     p.seg_off[s] = seg.off[s];
     p.seg_expert[s] = seg.expert[s];
     p.unit_start[s] = p.n_units;
-    if (seg.off[s + 1] > seg.off[s])
-      p.n_units += (seg.off[s + 1] - (seg.off[s] & ~63) + 255) / 256;
+    p.n_units += pair_units_of(seg, s);
   }
   p.seg_off[seg.nseg] = seg.off[seg.nseg];
   p.unit_start[seg.nseg] = p.n_units;
@@ -1032,27 +1044,10 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, int split, cudaStream_
              : 2;
 }
 
-// Row units of height h over the segments: blocks of h rows of the whole pass
-// (aligned) or of a segment from its first row rounded down to 64.
-inline int few_units(const SegInfo& seg, int h)
-{
-  int n = 0;
-  for (int s = 0; s < seg.nseg; ++s)
-    if (seg.off[s + 1] > seg.off[s]) n += (seg.off[s + 1] + h - 1) / h - seg.off[s] / h;
-  return n;
-}
-inline int pair_units(const SegInfo& seg)
-{
-  int n = 0;
-  for (int s = 0; s < seg.nseg; ++s)
-    if (seg.off[s + 1] > seg.off[s]) n += (seg.off[s + 1] - (seg.off[s] & ~63) + 255) / 256;
-  return n;
-}
-
 // The few-row form's cluster size (how many CTAs share a tile's k-blocks) with
-// the least time, and that time in nanoseconds as measured: rounds of the grid times (a
-// CTA's stages + its set-up and first loads), plus what the exchange of the
-// partial sums costs. resident[s]: the clusters of s CTAs that run at once,
+// the least time, and that time in nanoseconds as measured: rounds of the grid
+// times (a CTA's stages + its set-up, first loads and epilogue), plus what the
+// exchange of the partial sums costs. resident[s]: the clusters of s CTAs that run at once,
 // which the layout of the SMs makes fewer than SMs / s for most s.
 struct FewPlan {
   int split = 1;
@@ -1096,8 +1091,10 @@ const int* few_resident(int num_sms)
   for (int s = 1; s <= kMaxSplit; ++s) {
     attr[0].val.clusterDim.x = s;
     cfg.gridDim = dim3(s);
-    if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0)
+    if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0) {
+      cudaGetLastError();   // an estimate serves
       r[s] = std::max(1, num_sms / s / 2);
+    }
   }
   r[0] = 1;   // the entries are there
   return r;
@@ -1114,7 +1111,8 @@ FewPlan few_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* residen
 {
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   using C = FewCfg<MT, GU>;
-  const long tiles = (long)few_tiles<EPI>(a) * few_units(seg, MT);
+  long tiles = 0;
+  for (int s = 0; s < seg.nseg; ++s) tiles += (long)few_tiles<EPI>(a) * few_units_of(seg, s, MT);
   // a k-block of 128 weight rows: 160 ns, or 400 with 128 activation rows
   // beside them; a round's set-up, first loads and epilogue: 2.5 us and 20 ns a row
   const int stage_ns = C::kKps * C::kNA * (MT <= 64 ? 160 : 400);
@@ -1129,7 +1127,6 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cu
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   using C = FewCfg<MT, GU>;
   FewParams p{};
-  p.M = a.M;
   p.N = a.N;
   p.n_kblk = fp8_blocks(a.K);
   p.sf_blk_expert = (a.N + 127) / 128;
@@ -1144,7 +1141,7 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cu
     p.seg_off[s] = seg.off[s];
     p.seg_expert[s] = seg.expert[s];
     p.unit_start[s] = units;
-    if (seg.off[s + 1] > seg.off[s]) units += (seg.off[s + 1] + MT - 1) / MT - seg.off[s] / MT;
+    units += few_units_of(seg, s, MT);
   }
   p.seg_off[seg.nseg] = seg.off[seg.nseg];
   p.unit_start[seg.nseg] = units;
@@ -1180,7 +1177,8 @@ template <int EPI>
 int launch_many(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
 {
   const long n_st = (fp8_blocks(a.K) + kKps - 1) / kKps;
-  const long tiles = (long)pair_units(seg) * ((a.N + 255) / 256);
+  long tiles = 0;
+  for (int s = 0; s < seg.nseg; ++s) tiles += (long)pair_units_of(seg, s) * ((a.N + 255) / 256);
   const int* one = pair_resident<EPI, false>(a.num_sms);
   if (one == nullptr) return 2;
   // measured: 700 ns a stage of a pair and 5.5 us to start and finish; 850 ns
