@@ -62,8 +62,8 @@ __device__ __forceinline__ int seg_expert_of(int row, const SegInfo& s)
 // 128), and walk the rows with the grid's stride; a row stays in registers
 // between its sum of squares and its output. Sums in f32; s * w is exact
 // (two bf16), the mean and the reciprocal root are off by about half a unit, so
-// y carries little more than one f32 rounding ahead of its one to e4m3. x_out may be x or delta: every element
-// is read and written by one thread.
+// y carries little more than one f32 rounding ahead of its one to e4m3. x_out may
+// be x or delta: a row is read whole before any of it is written.
 // ---------------------------------------------------------------------
 
 // 1 / sqrt(v) to within about half a unit: the hardware's approximation and one
@@ -120,7 +120,8 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, norm_ctas<NT, KW>())
     const uint32_t n = (uint32_t)min(kRows, rows - r) * dim * 2;
     mbar_arrive_expect_tx(bar0 + 8 * s, delta != nullptr ? 2 * n : n);
     bulk_load(ring0 + s * stage, x + (long)r * dim, n, bar0 + 8 * s);
-    if (delta != nullptr) bulk_load(ring0 + s * stage + half, delta + (long)r * dim, n, bar0 + 8 * s);
+    if (delta != nullptr)
+      bulk_load(ring0 + s * stage + half, delta + (long)r * dim, n, bar0 + 8 * s);
   };
   const int first = blockIdx.x * kRows;
   if (threadIdx.x == 0) {
@@ -253,9 +254,9 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, norm_ctas<NT, KW>())
 
 // The same for rows too wide for registers: one CTA a row, which it reads twice.
 __global__ void __launch_bounds__(512)
-    add_norm_wide_fp8_kernel(const bf16* x, const bf16* delta, const bf16* __restrict__ w, bf16* x_out,
-                             uint8_t* __restrict__ q, uint8_t* __restrict__ scale, int dim,
-                             float2 inv_dim, float eps, SegInfo seg)
+    add_norm_wide_fp8_kernel(const bf16* x, const bf16* delta, const bf16* __restrict__ w,
+                             bf16* x_out, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
+                             int dim, float2 inv_dim, float eps, SegInfo seg)
 {
   griddep_launch();
   griddep_wait();
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(512)
     float t[8] = {}, g[8];
     if (c < dim) {
       // the sum from where it was stored: x or delta may be that place
-      unpack8f(x_out != nullptr ? *reinterpret_cast<const uint4*>(x_out + row * dim + c) : load(c), t);
+      unpack8f(x_out != nullptr ? *reinterpret_cast<const uint4*>(x_out + row * dim + c) : load(c),
+               t);
       unpack8f(__ldg(reinterpret_cast<const uint4*>(wr + c)), g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] = t[i] * g[i] * inv;
@@ -452,8 +454,8 @@ cudaError_t launch_norm(const bf16* x, const bf16* delta, const bf16* w, bf16* x
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k, x, delta, w, x_out, q, scale, rows, dim, inverse_of(dim), eps, seg,
-                            err);
+  return cudaLaunchKernelEx(&cfg, k, x, delta, w, x_out, q, scale, rows, dim, inverse_of(dim), eps,
+                            seg, err);
 }
 
 }  // namespace

@@ -24,8 +24,14 @@ namespace u15 {
 constexpr int kFp8Block = 128;       // columns (and weight rows) under one scale
 constexpr int kFp8SfTile = 512;      // bytes of a packed tile: 128 rows x 4 blocks
 
-__host__ __device__ __forceinline__ int fp8_blocks(int cols) { return (int)(((long)cols + 127) / 128); }
-__host__ __device__ __forceinline__ int fp8_groups(int cols) { return (int)(((long)cols + 511) / 512); }
+__host__ __device__ __forceinline__ int fp8_blocks(int cols)
+{
+  return (int)(((long)cols + 127) / 128);
+}
+__host__ __device__ __forceinline__ int fp8_groups(int cols)
+{
+  return (int)(((long)cols + 511) / 512);
+}
 __host__ __device__ __forceinline__ long fp8_scale_bytes(long rows, int cols)
 {
   return (rows + 127) / 128 * fp8_groups(cols) * kFp8SfTile;

@@ -44,7 +44,7 @@ constexpr int kTileBytes = 128 * 128;          // one operand, one k-block, one 
 constexpr int kStageBytes = 2 * kKps * kTileBytes + 2048;   // operands, then the scales
 constexpr int kSmemPair = kStg * kStageBytes + 1024 /*align*/ + 2048 /*amax*/ + 256 /*bars*/;
 constexpr int kThreadsPair = 320;
-constexpr int kMaxPairs = 4;                   // pairs a tile: clusters of 8 CTAs, the portable size
+constexpr int kMaxPairs = 4;   // pairs a tile: clusters of 8 CTAs, the portable size
 constexpr int kAccStep = 224;                  // accumulator 1 starts 32 columns early
 constexpr int kSfCol = 480;                    // two sets of 8 + 8 scale columns
 
@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
   const uint32_t amax0 = drain + 8;             // each CTA, a lane quadrant: 64 threads
 
   const uint32_t w = warp_id();
-  const uint32_t cta = cluster_ctarank(), rank = cta & 1, lead_cta = cta & ~1u;   // rank in the pair
+  // rank: in the pair
+  const uint32_t cta = cluster_ctarank(), rank = cta & 1, lead_cta = cta & ~1u;
   const bool leader = rank == 0;
   const uint16_t both = (uint16_t)(3u << lead_cta);   // the pair's CTAs, for commits
   if (threadIdx.x == 0) {

@@ -169,11 +169,6 @@ class CudaOps:
         n = n_experts * lib().u15c_fp8_scale_bytes(rows, cols)
         return torch.empty(n, dtype=torch.uint8, device=device)
 
-    @staticmethod
-    def _scale(what, t, rows, cols, n_experts=1):
-        return _need(what, t, n_experts * ((rows + 127) // 128) * _fp8_groups(cols) * 512,
-                     torch.uint8)
-
     def quant_rows_fp8(self, x, q, scale, rows, cols):
         n, d = rows * cols, _device()
         check(lib().u15c_quant_rows_fp8(_raw_stream(d), _need(d, "x", x, n, _BF16),
