@@ -376,7 +376,9 @@ def random_quantised(ops, rows, cols, seed, std):
     (1030, 272, 8192, [(0, 320, 0), (320, 1030, 1)]),
     # fewer tiles than pairs: two, three and four pairs a tile
     (512, 2064, 4096, [(0, 512, 0)]), (300, 12288, 2048, [(0, 300, 1)]),
-    (400, 8192, 1536, [(0, 100, 0), (100, 400, 1)]), (450, 2304, 4000, [(0, 130, 1), (130, 450, 0)])])
+    (400, 8192, 1536, [(0, 100, 0), (100, 400, 1)]), (450, 2304, 4000, [(0, 130, 1), (130, 450, 0)]),
+    (1100, 12288, 1024, [(0, 1100, 0)]), (1030, 2320, 1500, [(0, 70, 1), (70, 1030, 0)]),
+    (1300, 4096, 520, [(0, 700, 1), (700, 700, 0), (700, 1300, 0)])])
 @pytest.mark.parametrize("epi", [STORE, RESID, SWIGLU])
 def test_many_tiles(ops, M, K, N, segs, epi):
     """More tiles than CTA pairs: the accumulators' shared columns, the scale
@@ -406,6 +408,25 @@ def test_many_tiles(ops, M, K, N, segs, epi):
     assert ((y.double() - t).abs() <= err + 2.0 ** -8 * t.abs()).all()
 
 
+# Units of some hundred rows: their first rows rounded down to 64, their heights
+# to 32, so boundaries lie beside both; the last CTA past the columns; a last k-block alone
+# in its stage; the k-blocks of a tile split over up to four pairs
+EIGHT = [(0, 63, 0), (63, 64, 1), (64, 65, 0), (65, 161, 1), (161, 257, 0), (257, 257, 1),
+         (257, 450, 1), (450, 1024, 0)]
+
+
+@pytest.mark.parametrize("M,K,N,segs", [
+    (65, 16, 128, None), (66, 272, 129, [(0, 65, 1), (65, 66, 0)]),
+    (96, 400, 384, [(0, 32, 0), (32, 96, 1)]), (97, 1168, 640, [(0, 31, 1), (31, 97, 0)]),
+    (160, 640, 136, [(0, 64, 0), (64, 160, 1)]), (193, 4240, 256, [(0, 127, 1), (127, 193, 0)]),
+    (257, 8208, 392, None), (320, 2176, 260, [(0, 1, 1), (1, 320, 0)]),
+    (1000, 528, 768, [(0, 77, 0), (77, 1000, 1)]), (1024, 272, 1160, EIGHT), (1024, 1296, 513, None),
+    (1025, 1296, 513, None)])
+@pytest.mark.parametrize("epi", [STORE, RESID, F32])
+def test_linear_units(ops, M, K, N, segs, epi):
+    run_linear(ops, M, K, N, segs, epi, bias=epi != RESID)
+
+
 # ------------------------------------------------------------------ SwiGLU
 def swiglu_ref(xq, xs, W, M, K, segs):
     """silu(gate) * up of every row, and what f32 sums may be off by there."""
@@ -421,7 +442,9 @@ def swiglu_ref(xq, xs, W, M, K, segs):
 
 
 @pytest.mark.parametrize("M,K,I", [(1, 4096, 128), (1, 16, 256), (9, 640, 384), (33, 1040, 128),
-                                   (65, 512, 640), (128, 256, 256), (130, 144, 256), (300, 1024, 640)])
+                                   (65, 512, 640), (128, 256, 256), (130, 144, 256), (300, 1024, 640),
+                                   (70, 4240, 128), (190, 400, 384), (333, 1168, 896),
+                                   (1024, 272, 384)])
 @pytest.mark.parametrize("segs", ["one", "many"])
 def test_swiglu(ops, M, K, I, segs):
     segs = segments_of(M, segs)

@@ -158,18 +158,6 @@ __device__ __forceinline__ void add32(float (&v)[32], const bf16* src, int col0,
 
 // four columns of a row, of which the first n exist; `whole`: all four, and
 // rows are a multiple of four columns
-__device__ __forceinline__ void add4(float (&v)[4], const bf16* src, bool whole, int n)
-{
-  if (whole && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
-    const uint2 u = *reinterpret_cast<const uint2*>(src);
-    const float2 a = unpack_bf2(u.x), b = unpack_bf2(u.y);
-    v[0] += a.x; v[1] += a.y; v[2] += b.x; v[3] += b.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) v[i] += bf2f(src[i]);
-  }
-}
 __device__ __forceinline__ void store4(bf16* dst, const float (&v)[4], bool whole, int n)
 {
   if (whole && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
@@ -191,11 +179,47 @@ __device__ __forceinline__ void store4(float* dst, const float (&v)[4], bool who
   }
 }
 
+// What is added to four columns of R rows, `step` rows apart from `row` on: their
+// residual or the bias, as the bits of four bf16. All of a step's rows are read, and
+// nothing waits for them, before the first is stored: y may be the residual, so no
+// load passes a store, and row after row each load's wait showed (256 rows of 128
+// columns: 7.4 us).
+template <int EPI, int R, class P>
+__device__ __forceinline__ void addend4(uint2 (&a)[R], const P& p, long row, int step, int n_rows,
+                                        int expert, int col, int ncols)
+{
+  if constexpr (EPI == kEpiResid || EPI == kEpiStore || EPI == kEpiStoreF32) {
+    const bf16* src = p.resid + row * ncols + col;
+    long pitch = (long)step * ncols;
+    if (EPI != kEpiResid) {
+      if (p.bias == nullptr) return;
+      src = p.bias + (long)expert * p.N + col;
+      pitch = 0;
+    }
+    // four columns, aligned together
+    if (col + 4 <= ncols && (ncols & 3) == 0 && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (i < n_rows) a[i] = *reinterpret_cast<const uint2*>(src + i * pitch);
+    } else {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        uint32_t x[4] = {};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i < n_rows && col + k < ncols) x[k] = u[i * pitch + k];
+        a[i] = make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
+      }
+    }
+  }
+}
+
 // Four finished columns of a row, at column `col` of ncols, a warp a run of 128
 // (with SwiGLU applied): the epilogue's other steps and the store. `blk`: the
 // block of 128 outputs of a quantised row.
 template <int EPI, class P>
-__device__ __forceinline__ void finish4(float (&v)[4], const P& p, long row, int blk, int expert,
+__device__ __forceinline__ void finish4(float (&v)[4], uint2 a, const P& p, long row, int blk,
                                         int col, int ncols)
 {
   if constexpr (EPI == kEpiSwigluFp8) {
@@ -209,14 +233,30 @@ __device__ __forceinline__ void finish4(float (&v)[4], const P& p, long row, int
     if (lane_id() == 0) p.sy[fp8_scale_at(row, blk, fp8_groups(ncols))] = (uint8_t)sb;
   } else {
     const long at = row * ncols + col;
-    const bool whole = col + 4 <= ncols && (ncols & 3) == 0;   // four columns, aligned together
-    if (p.bias != nullptr) add4(v, p.bias + (long)expert * p.N + col, whole, ncols - col);
-    if constexpr (EPI == kEpiResid) add4(v, p.resid + at, whole, ncols - col);
+    const bool whole = col + 4 <= ncols && (ncols & 3) == 0;
+    if (EPI == kEpiResid || ((EPI == kEpiStore || EPI == kEpiStoreF32) && p.bias != nullptr)) {
+      const float2 lo = unpack_bf2(a.x), hi = unpack_bf2(a.y);
+      v[0] += lo.x;
+      v[1] += lo.y;
+      v[2] += hi.x;
+      v[3] += hi.y;
+    }
     if constexpr (EPI == kEpiStoreF32)
       store4(static_cast<float*>(p.y) + at, v, whole, ncols - col);
     else
       store4(static_cast<bf16*>(p.y) + at, v, whole, ncols - col);
   }
+}
+
+// Sends the residual of the rows first + k * step < end, `cols` columns from `col`
+// on, towards L2, a row a thread: the epilogue reads them when the products are done.
+template <class P>
+__device__ __forceinline__ void prefetch_resid(const P& p, int first, int step, int end, int n_thr,
+                                               int thr, int col, int cols)
+{
+  for (int j = first + thr * step; j < end; j += n_thr * step)
+    for (int c = col; c < min(col + cols, p.N); c += 64)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.resid + (long)j * p.N + c));
 }
 
 template <int EPI, bool SPLIT>
@@ -553,6 +593,13 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
       auto finish = [&](auto r_, auto q_) {
         constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
         for (int j0 = lo + part + (int)w * p.split; j0 < hi; j0 += R * step) {
+          uint2 a[2][R] = {};
+          if constexpr (!GU) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              addend4<EPI>(a[h], p, first + j0, step, (hi - j0 + step - 1) / step, ti.expert,
+                           ti.nb * 256 + h * 128 + lane * 4, p.N);
+          }
           float4 v[Q][R][2] = {};
 #pragma unroll
           for (int q = 0; q < Q; ++q) {
@@ -573,28 +620,28 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
             float t[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float4 a = v[0][i][h];
+              float4 x = v[0][i][h];
 #pragma unroll
               for (int q = 1; q < Q; ++q) {
-                a.x += v[q][i][h].x;
-                a.y += v[q][i][h].y;
-                a.z += v[q][i][h].z;
-                a.w += v[q][i][h].w;
+                x.x += v[q][i][h].x;
+                x.y += v[q][i][h].y;
+                x.z += v[q][i][h].z;
+                x.w += v[q][i][h].w;
               }
-              t[h][0] = a.x;
-              t[h][1] = a.y;
-              t[h][2] = a.z;
-              t[h][3] = a.w;
+              t[h][0] = x.x;
+              t[h][1] = x.y;
+              t[h][2] = x.z;
+              t[h][3] = x.w;
             }
             const long row = first + j0 + i * step;
             if constexpr (GU) {
 #pragma unroll
               for (int k = 0; k < 4; ++k) t[0][k] = swiglu1(t[0][k], t[1][k]);
-              finish4<EPI>(t[0], p, row, ti.nb, ti.expert, ti.nb * 128 + lane * 4, p.N / 2);
+              finish4<EPI>(t[0], a[0][i], p, row, ti.nb, ti.nb * 128 + lane * 4, p.N / 2);
             } else {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                finish4<EPI>(t[h], p, row, ti.nb, ti.expert, ti.nb * 256 + h * 128 + lane * 4, p.N);
+                finish4<EPI>(t[h], a[h][i], p, row, ti.nb, ti.nb * 256 + h * 128 + lane * 4, p.N);
             }
           }
         }
@@ -635,7 +682,6 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 //              cluster and the epilogue, a row a warp
 // ---------------------------------------------------------------------
 constexpr int kThreadsFew = 192;
-constexpr int kFewRows = 1024;      // rows up to which this form is considered
 constexpr int kFewPrefetch = 4;     // k-blocks a CTA sends towards L2 ahead of its loads
 constexpr int kMaxSplit = 8;        // the portable cluster size
 
@@ -832,6 +878,8 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   const int wq = (int)(w & 3), n = wq * 32 + (int)lane_id();
   bool ok = true;
   if (w >= 2) {
+    if constexpr (EPI == kEpiResid)
+      prefetch_resid(p, m0 + lo + rank, split, m0 + hi, 128, (int)threadIdx.x - 64, tile * 128, 128);
     // every MMA of this CTA has completed, and with them every load
     ok = warp_wait(accf, 0, p.err, kDevWaitAccFull);
     tc_fence_after();
@@ -858,12 +906,15 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
     // 128 rows of an unsplit tile took 5 us; four rows from two CTAs at a time,
     // eight CTAs' sums 2 us more)
     constexpr int kWarps = kThreadsFew / 32;
-    const uint32_t own = smem_u32(part) + lane_id() * 16;
+    const float4* mine = reinterpret_cast<const float4*>(part) + lane_id();
+    const uint32_t own = smem_u32(mine);
     const int ncols = GU ? p.N / 2 : p.N, col = tile * 128 + (int)lane_id() * 4;
     const int step = kWarps * split;
     auto finish = [&](auto r_, auto q_) {
       constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
       for (int j0 = lo + rank + (int)w * split; j0 < hi; j0 += R * step) {
+        uint2 a[R] = {};
+        addend4<EPI>(a, p, m0 + j0, step, (hi - j0 + step - 1) / step, expert, col, ncols);
         float4 v[Q][NA][R] = {};
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
@@ -873,8 +924,13 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
           for (int h = 0; h < NA; ++h)
 #pragma unroll
             for (int i = 0; i < R; ++i)
-              if (j0 + i * step < hi)
-                v[q][h][i] = ld_cluster4(from + (h * MT + j0 + i * step) * 512);
+              if (j0 + i * step < hi) {
+                const int at = h * MT + j0 + i * step;
+                if constexpr (Q == 1)
+                  v[q][h][i] = mine[at * 32];
+                else
+                  v[q][h][i] = ld_cluster4(from + at * 512);
+              }
         }
         float4 t[NA][R];
 #pragma unroll
@@ -900,12 +956,14 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
             v[2] = swiglu1(v[2], t[1][i].z);
             v[3] = swiglu1(v[3], t[1][i].w);
           }
-          finish4<EPI>(v, p, m0 + j0 + i * step, tile, expert, col, ncols);
+          finish4<EPI>(v, a[i], p, m0 + j0 + i * step, tile, col, ncols);
         }
       }
     };
     using std::integral_constant;
-    if (split <= 2)
+    if (split == 1)
+      finish(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    else if (split == 2)
       finish(integral_constant<int, 4>{}, integral_constant<int, 2>{});
     else
       finish(integral_constant<int, 1>{}, integral_constant<int, kMaxSplit>{});
@@ -917,6 +975,315 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   if (w == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+// ---------------------------------------------------------------------
+// Some hundred rows: 256-row tiles would compute rows that are not there, and
+// the few-row form loads the activations beside every 128 weight rows. Here a
+// CTA pair's M = 256 side is weights, 128 rows (SwiGLU: 128 gate and 128 up
+// rows) a CTA, and its N side a unit of up to kRows activation rows, as many as the
+// segment has there rounded up to 32, half of them loaded by each CTA. A
+// CTA's accumulator then is its own 128 columns of all the unit's rows, and
+// the epilogue is the few-row form's. The k-blocks of a tile are split over the
+// pairs of a cluster.
+//   warp 0     TMA producer (both CTAs)
+//   warp 1     MMA issuer (leader)
+//   warps 2-9  TMEM -> shared memory; then every warp: the sum over the
+//              cluster's pairs and the epilogue, a row a warp
+// ---------------------------------------------------------------------
+constexpr int kThreadsMid = 320;
+constexpr int kMidRows = 1024;      // rows up to which this form is considered
+constexpr int kMidUnits = 40;       // units of a pass: 1024 rows / 64, and two ends a segment
+
+template <bool GU>
+struct MidCfg {
+  static constexpr int kNA = GU ? 2 : 1;
+  static constexpr int kRows = GU ? 192 : 256;              // of a unit: TMEM holds NA x kRows
+  static constexpr int kXTiles = GU ? 2 : 3;                // scale tiles that its rows lie in
+  static constexpr int kKps = GU ? 1 : 2;                   // k-blocks per stage
+  static constexpr int kA = kNA * kTileBytes;               // a k-block, a CTA
+  static constexpr int kMaxStages = 6;
+  static constexpr int kBody = 225 * 1024;                  // the ring, then the partial sums
+  static constexpr int kSmem = kBody + 1024 /*align*/ + 256 /*bars*/;
+  static constexpr int kAcc = kNA * kRows;
+  static constexpr int kSf = 4 * (kNA + kXTiles);           // scale columns of a set, two sets
+  // a stage's bytes: operands (xr activation rows a CTA), then the scale tiles
+  __host__ __device__ static constexpr int stage(int xr) { return kKps * (kA + xr * 128) + 2048; }
+  static_assert(kAcc + 2 * kSf <= 512 && (kNA + kXTiles) * kFp8SfTile <= 2048 && kSmem <= 232448);
+  static_assert(3 * stage(kRows / 2) <= kBody && kNA * kRows * 512 <= kBody);
+};
+
+struct MidUnit {
+  int m0, expert;   // first row, a multiple of 64
+  short lo, hi;     // rows [m0 + lo, m0 + hi) are the segment's
+};
+
+struct MidParams {
+  int N, n_kblk;
+  int sf_blk_expert;
+  void* y;
+  const bf16* resid;
+  const bf16* bias;
+  uint8_t* sy;
+  unsigned* err;
+  MidUnit unit[kMidUnits];
+};
+
+template <int EPI>
+__global__ void __launch_bounds__(kThreadsMid, 1)
+    gemm_fp8_mid_kernel(const __grid_constant__ CUtensorMap tmX,
+                        const __grid_constant__ CUtensorMap tmW,
+                        const __grid_constant__ CUtensorMap tmSX,
+                        const __grid_constant__ CUtensorMap tmSW,
+                        const __grid_constant__ MidParams p)
+{
+  constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
+  using C = MidCfg<GU>;
+  constexpr int NA = C::kNA;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBody);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::kMaxStages + 2);
+  const uint32_t full0 = smem_u32(bars);               // leader: count 2 (one per CTA) + tx
+  const uint32_t empty0 = full0 + 8 * C::kMaxStages;   // each CTA: leader's multicast commit
+  const uint32_t accf = empty0 + 8 * C::kMaxStages, drain = accf + 8;   // the same
+
+  griddep_launch();
+  const uint32_t w = warp_id();
+  const uint32_t cta = cluster_ctarank(), rank = cta & 1, lead_cta = cta & ~1u;
+  const uint16_t both = (uint16_t)(3u << lead_cta);
+  const int split = (int)gridDim.x >> 1, part_k = (int)(cta >> 1);   // the cluster is the x axis
+  const int blk = (int)blockIdx.y * 2 + (int)rank;   // this CTA's 128 output columns
+  const MidUnit u = p.unit[blockIdx.z];
+  const int nr = (u.hi + 31) & ~31;                  // rows the MMAs take
+  const int xr = ((nr >> 1) + 31) & ~31;             // rows a CTA loads, in boxes of 32
+  // this CTA's stages of the tile, and their first k-block
+  const int n_st = (p.n_kblk + C::kKps - 1) / C::kKps, st0 = part_k * n_st / split;
+  const int n_it = (part_k + 1) * n_st / split - st0, kb0 = st0 * C::kKps;
+  // the ring: as many stages of this unit's size as fit
+  const int stage = C::stage(xr), n_ring = min(C::kMaxStages, C::kBody / stage);
+  const uint32_t base = smem_u32(smem);
+  // scale tiles of the unit's rows, and the scale column of its first (0 or 2)
+  const int x_tiles = ((u.m0 & 127) + nr + 127) >> 7, x_col = (u.m0 >> 5) & 3;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < n_ring; ++s) {
+      mbar_init(full0 + 8 * s, 2);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    mbar_init(accf, 1);
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (w == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  const int wrow = u.expert * p.N + blk * 128 * NA;
+  if (threadIdx.x == 64) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmSW);
+    tma_prefetch_desc(&tmSX);
+    // as in the few-row form, while the previous kernel still runs
+    for (int i = 0; i < min(kFewPrefetch, min(n_it * C::kKps, p.n_kblk - kb0)); ++i)
+      for (int h = 0; h < NA; ++h) tma_prefetch_2d(&tmW, (kb0 + i) * 128, wrow + 128 * h);
+  }
+  tc_fence_before();
+  cluster_sync();   // barriers of both CTAs initialised before any remote arrive
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+
+  if (w == 0) {
+    int it = 0;
+    for (int s = 0, ph = 0; it < n_it; ++it) {
+      if (!warp_wait_probe(empty0 + 8 * s, ph ^ 1, p.err, kDevWaitEmpty)) break;
+      const int kb = kb0 + it * C::kKps, nk = min(C::kKps, p.n_kblk - kb);
+      const uint32_t st = base + s * stage, fb = mapa_shared(full0 + 8 * s, lead_cta);
+      const bool sfs = it == 0 || (kb & 3) == 0;   // a scale tile serves its four k-blocks
+      if (elect_one()) {
+        mbar_arrive_expect_tx_cluster(
+            fb, nk * (C::kA + xr * 128) + (sfs ? (NA + x_tiles) * kFp8SfTile : 0));
+        if (sfs) {
+          const uint32_t sf = st + C::kKps * (C::kA + xr * 128);
+#pragma unroll
+          for (int h = 0; h < NA; ++h)
+            tma_load_sf_pair(sf + h * kFp8SfTile, &tmSW, kb >> 2,
+                             u.expert * p.sf_blk_expert + blk * NA + h, fb);
+          for (int i = 0; i < x_tiles; ++i)
+            tma_load_sf_pair(sf + (NA + i) * kFp8SfTile, &tmSX, kb >> 2, (u.m0 >> 7) + i, fb);
+        }
+        const int x0 = u.m0 + (int)rank * (nr >> 1);
+#pragma unroll
+        for (int hk = 0; hk < C::kKps; ++hk) {
+          if (hk >= nk) break;
+          const int kx = (kb + hk) * 128;
+#pragma unroll
+          for (int h = 0; h < NA; ++h)
+            tma_load_2d_pair(st + (hk * NA + h) * kTileBytes, &tmW, kx, wrow + 128 * h, fb);
+          const uint32_t xb = st + C::kKps * C::kA + hk * xr * 128;
+          for (int i = 0; i < xr; i += 32) tma_load_2d_pair(xb + i * 128, &tmX, kx, x0 + i, fb);
+        }
+      }
+      __syncwarp();
+      if (++s == n_ring) s = 0, ph ^= 1;
+    }
+    // the leader: the last fill of every stage, both CTAs' halves, has landed
+    if (rank == 0)
+      for (int s = 0; s < n_ring; ++s)
+        if (it > s) warp_wait(full0 + 8 * s, ((it - 1 - s) / n_ring) & 1, p.err, kDevWaitDrain);
+  } else if (w == 1) {
+    if (rank == 0) {
+      const uint32_t idesc = idesc_e4m3(256, nr);
+      uint32_t set = 0;
+      bool ok = true;
+      for (int it = 0, s = 0, ph = 0; it < n_it; ++it) {
+        if (!warp_wait_probe(full0 + 8 * s, ph, p.err, kDevWaitFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int kb = kb0 + it * C::kKps, nk = min(C::kKps, p.n_kblk - kb);
+        const uint32_t st = base + s * stage;
+        const bool sfs = it == 0 || (kb & 3) == 0;
+        set ^= sfs;
+        const uint32_t sfw = tmem + C::kAcc + set * C::kSf, sfx = sfw + 4 * NA;
+        const uint64_t ad = smem_desc_sw128(st), bd = smem_desc_sw128(st + C::kKps * C::kA);
+        if (elect_one()) {
+          if (sfs) {
+            const uint64_t sf = smem_desc_sf(st + C::kKps * (C::kA + xr * 128));
+            for (int i = 0; i < NA + x_tiles; ++i)
+              sf_copy_pair(sfw + 4 * i, sf + i * (kFp8SfTile >> 4));
+          }
+#pragma unroll
+          for (int hk = 0; hk < C::kKps; ++hk) {
+            if (hk >= nk) break;
+            const uint32_t id = idesc | idesc_scale_byte((kb + hk) & 3);
+            // K = 32 steps are 32 bytes, 2 descriptor units, apart
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int h = 0; h < NA; ++h)
+                mma_e4m3_pair(tmem + h * C::kRows, ad + (hk * NA + h) * (kTileBytes >> 4) + k * 2,
+                              bd + hk * xr * 8 + k * 2, id, sfw + 4 * h, sfx + x_col,
+                              (it | hk | k) != 0);
+          }
+          mma_commit_pair_mc(empty0 + 8 * s, both);
+        }
+        __syncwarp();
+        if (++s == n_ring) s = 0, ph ^= 1;
+      }
+      if (elect_one()) {
+        if (ok) mma_commit_pair_mc(accf, both);
+        mma_commit_pair_mc(drain, both);
+      }
+      __syncwarp();
+    }
+    // both CTAs: every MMA that writes this CTA's TMEM has completed
+    warp_wait(drain, 0, p.err, kDevWaitDrain);
+  }
+
+  float* part = reinterpret_cast<float*>(smem);   // [NA][rows][128 columns], over the ring
+  bool ok = true;
+  if (w >= 2) {
+    if constexpr (EPI == kEpiResid)
+      prefetch_resid(p, u.m0 + u.lo + part_k, split, u.m0 + u.hi, 256, (int)threadIdx.x - 64,
+                     blk * 128, 128);
+    // every MMA of the pair has completed, and with them every load of both CTAs
+    ok = warp_wait(accf, 0, p.err, kDevWaitAccFull);
+    tc_fence_after();
+    const int wq = (int)(w & 3), n = wq * 32 + (int)lane_id();
+    const uint32_t tb = tmem + ((uint32_t)(wq * 32) << 16);
+#pragma unroll 1
+    for (int c = (u.lo & ~15) + ((int)(w - 2) >> 2) * 16; c < u.hi && ok; c += 32) {
+#pragma unroll
+      for (int h = 0; h < NA; ++h) {
+        uint32_t r[16];
+        tmem_ld16(tb + h * C::kRows + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          part[(h * C::kRows + c + i) * 128 + n] = __uint_as_float(r[i]);
+      }
+    }
+  }
+  __syncthreads();
+  if (split > 1) cluster_sync();   // every pair's partial sums are in its shared memory
+
+  const int ncols = GU ? p.N / 2 : p.N, col = blk * 128 + (int)lane_id() * 4;
+  if (ok && blk * 128 < ncols) {   // the last pair's second CTA may be past the columns
+    constexpr int kWarps = kThreadsMid / 32;
+    const float4* mine = reinterpret_cast<const float4*>(part) + lane_id();
+    const uint32_t own = smem_u32(mine);
+    const int step = kWarps * split;
+    auto finish = [&](auto r_, auto q_) {
+      constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
+      for (int j0 = u.lo + part_k + (int)w * split; j0 < u.hi; j0 += R * step) {
+        uint2 a[R] = {};
+        addend4<EPI>(a, p, u.m0 + j0, step, (u.hi - j0 + step - 1) / step, u.expert, col, ncols);
+        float4 v[Q][NA][R] = {};
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          if (q >= split) break;
+          const uint32_t from = mapa_shared(own, 2 * q + rank);
+#pragma unroll
+          for (int h = 0; h < NA; ++h)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+              if (j0 + i * step < u.hi) {
+                const int at = h * C::kRows + j0 + i * step;
+                if constexpr (Q == 1)
+                  v[q][h][i] = mine[at * 32];
+                else
+                  v[q][h][i] = ld_cluster4(from + at * 512);
+              }
+        }
+        float4 t[NA][R];
+#pragma unroll
+        for (int h = 0; h < NA; ++h)
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            t[h][i] = v[0][h][i];
+#pragma unroll
+            for (int q = 1; q < Q; ++q) {
+              t[h][i].x += v[q][h][i].x;
+              t[h][i].y += v[q][h][i].y;
+              t[h][i].z += v[q][h][i].z;
+              t[h][i].w += v[q][h][i].w;
+            }
+          }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (j0 + i * step >= u.hi) break;
+          float o[4] = {t[0][i].x, t[0][i].y, t[0][i].z, t[0][i].w};
+          if constexpr (GU) {
+            o[0] = swiglu1(o[0], t[1][i].x);
+            o[1] = swiglu1(o[1], t[1][i].y);
+            o[2] = swiglu1(o[2], t[1][i].z);
+            o[3] = swiglu1(o[3], t[1][i].w);
+          }
+          finish4<EPI>(o, a[i], p, u.m0 + j0 + i * step, blk, col, ncols);
+        }
+      }
+    };
+    using std::integral_constant;
+    if (split == 1)
+      finish(integral_constant<int, 8 / NA>{}, integral_constant<int, 1>{});
+    else if (split == 2)
+      finish(integral_constant<int, 4 / NA>{}, integral_constant<int, 2>{});
+    else
+      finish(integral_constant<int, 2 / NA>{}, integral_constant<int, kMaxPairs>{});
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_relaxed();   // the peers have read this CTA's partial sums, and its TMEM is idle
+  if (w == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -1114,9 +1481,9 @@ FewPlan few_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* residen
   using C = FewCfg<MT, GU>;
   long tiles = 0;
   for (int s = 0; s < seg.nseg; ++s) tiles += (long)few_tiles<EPI>(a) * few_units_of(seg, s, MT);
-  // a k-block of 128 weight rows: 160 ns, or 400 with 128 activation rows
-  // beside them; a round's set-up, first loads and epilogue: 2.5 us and 20 ns a row
-  const int stage_ns = C::kKps * C::kNA * (MT <= 64 ? 160 : 400);
+  // a k-block of 128 weight rows: 160 ns; a round's set-up, first loads and
+  // epilogue: 2.5 us and 20 ns a row
+  const int stage_ns = C::kKps * C::kNA * 160;
   return few_plan(tiles, (fp8_blocks(a.K) + C::kKps - 1) / C::kKps, stage_ns, 2500 + 20 * MT,
                   resident);
 }
@@ -1173,7 +1540,166 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cu
              : 2;
 }
 
-// More than 64 rows: tiles of 256 rows (pairs, one or several a tile) or of 128.
+// Clusters of 1 to kMaxPairs pairs of the form above that can be resident.
+template <int EPI>
+const int* mid_resident(int num_sms)
+{
+  using C = MidCfg<EPI == kEpiSwiglu || EPI == kEpiSwigluFp8>;
+  static std::atomic<uint64_t> attr_set;
+  static std::mutex mu;
+  static int resident_dev[64][kMaxPairs + 1];
+  auto k = gemm_fp8_mid_kernel<EPI>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || !smem_attr_once(k, C::kSmem, attr_set)) return nullptr;
+  std::lock_guard<std::mutex> g(mu);
+  int* r = resident_dev[dev & 63];
+  if (r[0] != 0) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreadsMid);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  for (int s = 1; s <= kMaxPairs; ++s) {
+    attr[0].val.clusterDim.x = 2 * s;
+    cfg.gridDim = dim3(2 * s);
+    if (cudaOccupancyMaxActiveClusters(&r[s], k, &cfg) != cudaSuccess || r[s] <= 0) {
+      cudaGetLastError();   // an estimate serves
+      r[s] = std::max(1, num_sms / (4 * s));
+    }
+  }
+  r[0] = 1;   // the entries are there
+  return r;
+}
+
+struct MidPlan {
+  int height = 64, split = 1;   // rows of a unit, pairs a tile
+  long ns = -1;
+};
+
+// The units of height `h`, tallest first (the last round then holds the small
+// ones), and how many they are.
+inline int mid_units(const SegInfo& seg, int h, MidUnit* unit)
+{
+  int n = 0;
+  for (int s = 0; s < seg.nseg; ++s) {
+    const int end = seg.off[s + 1];
+    if (end <= seg.off[s]) continue;
+    for (int m0 = seg.off[s] & ~63; m0 < end; m0 += h, ++n)
+      unit[n] = MidUnit{m0, seg.expert[s], (short)std::max(0, seg.off[s] - m0),
+                        (short)std::min(h, end - m0)};
+  }
+  std::sort(unit, unit + n, [](const MidUnit& a, const MidUnit& b) { return a.hi > b.hi; });
+  return n;
+}
+
+template <int EPI>
+int mid_tiles(const GemmFp8Args& a)
+{
+  return EPI == kEpiSwiglu || EPI == kEpiSwigluFp8 ? (a.N + 511) / 512 : (a.N + 255) / 256;
+}
+
+// Nanoseconds of a k-block of a unit of nr rows, and of its set-up, first loads and
+// epilogue, as measured (4096 columns of one unit, K 512 to 12288: 64 rows 4.7 to
+// 19.7 us, 128 6.0 to 22.5, 256 9.3 to 35.8; the SwiGLU form's two accumulators, K
+// 512 and 2048: 128 rows 9.7 and 13.6, 192 13.1 and 18.8).
+// With many CTAs at it the SwiGLU form's loads count (two weight tiles a k-block):
+// 12.3 TB/s into all of the chip's shared memory.
+template <bool GU>
+inline long mid_kblk_ns(int nr, int ctas)
+{
+  if (!GU) return std::max(160, 90 + 3 * nr / 4);
+  const long bytes = MidCfg<GU>::kA + nr * 64;
+  return std::max<long>(std::max(280, 5 * nr / 2), ctas * bytes / 12300);
+}
+template <bool GU>
+inline long mid_unit_ns(int nr)
+{
+  return GU ? 2800 + 44 * nr : 2700 + 21 * nr;
+}
+
+template <int EPI>
+MidPlan mid_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* resident)
+{
+  constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
+  const int n_kblk = fp8_blocks(a.K), tiles = mid_tiles<EPI>(a);
+  MidPlan best;
+  for (int h = 64; h <= MidCfg<GU>::kRows; h += 64) {
+    MidUnit unit[kMidUnits];
+    const int n = mid_units(seg, h, unit);
+    for (int s = 1; s <= kMaxPairs && s <= n_kblk; ++s) {
+      // tile i's time, the tiles in order of their units' heights
+      const long places = resident[s], all = (long)tiles * n;
+      auto time = [&](long i) {
+        const int nr = (unit[i / tiles].hi + 31) & ~31;
+        const int ctas = 2 * s * (int)std::min(places, all);
+        return (n_kblk + s - 1) / s * mid_kblk_ns<GU>(nr, ctas) + mid_unit_ns<GU>(nr);
+      };
+      // rounds of as many tiles as run at once, each the time of its first; of the
+      // last two, the later one's tiles start as the smallest before them end
+      long ns = s > 1 ? 1000 + 300 * s : 0, t0 = 0;
+      for (; all - t0 > 2 * places; t0 += places) ns += time(t0);
+      const long late = all - t0 - places;
+      ns += late <= 0 ? time(t0)
+                      : std::max({time(t0), time(t0 + places - 1) + time(t0 + places),
+                                  time(t0 + places - late) + time(all - 1)});
+      if (best.ns < 0 || ns < best.ns) {
+        best.height = h;
+        best.split = s;
+        best.ns = ns;
+      }
+    }
+  }
+  return best;
+}
+
+template <int EPI>
+int launch_mid(const GemmFp8Args& a, const SegInfo& seg, const MidPlan& plan, cudaStream_t st,
+               std::string* err)
+{
+  using C = MidCfg<EPI == kEpiSwiglu || EPI == kEpiSwigluFp8>;
+  MidParams p{};
+  p.N = a.N;
+  p.n_kblk = fp8_blocks(a.K);
+  p.sf_blk_expert = (a.N + 127) / 128;
+  p.y = a.y;
+  p.resid = static_cast<const bf16*>(a.resid);
+  p.bias = static_cast<const bf16*>(a.bias);
+  p.sy = a.sy;
+  p.err = a.dev_err;
+  const int units = mid_units(seg, plan.height, p.unit);
+  CUtensorMap mx, mw, msx, msw;
+  const uint64_t groups = fp8_groups(a.K);
+  if (make_tma_2d(&mx, a.xq, a.M, a.K, 32, 1, err) ||
+      make_tma_2d(&mw, a.wq, (uint64_t)a.N * a.n_experts, a.K, 128, 1, err) ||
+      make_tma_fp8_scales(&msx, a.sx, (a.M + 127) / 128, groups, 1, err) ||
+      make_tma_fp8_scales(&msw, a.sw, (uint64_t)p.sf_blk_expert * a.n_experts, groups, 1, err))
+    return 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreadsMid);
+  cfg.gridDim = dim3(2 * plan.split, mid_tiles<EPI>(a), units);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attrs[2] = {};
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = 2 * plan.split;
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_mid_kernel<EPI>, mx, mw, msx, msw, p) == cudaSuccess ? 0
+                                                                                               : 2;
+}
+
+// More than 64 rows: tiles of 256 rows (pairs, one or several a tile), or up to 1024
+// rows units of the rows there are, whichever form takes less time by the models
+// above (333 rows in two segments x 4096 x 12288: 28 us, in tiles of 256 or
+// 128 rows 40; 1000 rows 52 and 62; 100 rows x 6144 x 4096: 13 to 16 and 16 to 21).
 template <int EPI>
 int launch_many(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
 {
@@ -1182,12 +1708,15 @@ int launch_many(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
   for (int s = 0; s < seg.nseg; ++s) tiles += (long)pair_units_of(seg, s) * ((a.N + 255) / 256);
   const int* one = pair_resident<EPI, false>(a.num_sms);
   if (one == nullptr) return 2;
-  // measured: 700 ns a stage of a pair and 5.5 us to start and finish; 850 ns
-  // and 8.5 us where partial sums meet (512 rows x 4096 x 12288: one pair a
-  // tile 37 us, two 29.5, tiles of 128 rows 40; 256 rows: 37, three pairs 23.5,
-  // tiles of 128 rows 22.6; 256 x 24576 x 4096 SwiGLU: 30 and 57)
+  // measured: 790 ns a stage of a pair and 5.5 us to start and finish, a last
+  // round of half-width tiles half a round (launch_pair); 850 ns and 8.5 us where
+  // partial sums meet
+  constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   int split = 1;
-  long pair_ns = (tiles + one[1] - 1) / one[1] * n_st * 700 + 5500;
+  const long rest = tiles % one[1];
+  const long halves = 2 * (tiles / one[1]) +
+                      (rest == 0 ? 0 : !GU && tiles > one[1] && 2 * rest <= one[1] ? 1 : 2);
+  long pair_ns = halves * n_st * 395 + 5500;
   if (tiles < one[1]) {
     const int* more = pair_resident<EPI, true>(a.num_sms);
     if (more == nullptr) return 2;
@@ -1199,11 +1728,11 @@ int launch_many(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
       }
     }
   }
-  if (a.M <= kFewRows && few_tiles<EPI>(a) <= 65535) {
-    const int* resident = few_resident<128, EPI>(a.num_sms);
+  if (a.M <= kMidRows && mid_tiles<EPI>(a) <= 65535) {
+    const int* resident = mid_resident<EPI>(a.num_sms);
     if (resident == nullptr) return 2;
-    const FewPlan few = few_plan_of<128, EPI>(a, seg, resident);
-    if (few.ns < pair_ns) return launch_few<128, EPI>(a, seg, few, st, err);
+    const MidPlan mid = mid_plan_of<EPI>(a, seg, resident);
+    if (mid.ns < pair_ns) return launch_mid<EPI>(a, seg, mid, st, err);
   }
   return split > 1 ? launch_pair<EPI, true>(a, seg, split, st, err)
                    : launch_pair<EPI, false>(a, seg, 1, st, err);
