@@ -262,6 +262,16 @@ __device__ __forceinline__ void cluster_sync_relaxed()
 {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
+// 16 bytes of this CTA's shared memory
+__device__ __forceinline__ float4 ld_shared4(uint32_t addr)
+{
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
 // 16 bytes of another CTA of the cluster's shared memory
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr)
 {

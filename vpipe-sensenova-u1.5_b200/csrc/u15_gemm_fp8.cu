@@ -906,8 +906,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
     // 128 rows of an unsplit tile took 5 us; four rows from two CTAs at a time,
     // eight CTAs' sums 2 us more)
     constexpr int kWarps = kThreadsFew / 32;
-    const float4* mine = reinterpret_cast<const float4*>(part) + lane_id();
-    const uint32_t own = smem_u32(mine);
+    const uint32_t own = smem_u32(part) + lane_id() * 16;
     const int ncols = GU ? p.N / 2 : p.N, col = tile * 128 + (int)lane_id() * 4;
     const int step = kWarps * split;
     auto finish = [&](auto r_, auto q_) {
@@ -926,10 +925,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
             for (int i = 0; i < R; ++i)
               if (j0 + i * step < hi) {
                 const int at = h * MT + j0 + i * step;
-                if constexpr (Q == 1)
-                  v[q][h][i] = mine[at * 32];
-                else
-                  v[q][h][i] = ld_cluster4(from + at * 512);
+                v[q][h][i] = Q == 1 ? ld_shared4(own + at * 512) : ld_cluster4(from + at * 512);
               }
         }
         float4 t[NA][R];
@@ -989,10 +985,12 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
 // pairs of a cluster.
 //   warp 0     TMA producer (both CTAs)
 //   warp 1     MMA issuer (leader)
-//   warps 2-9  TMEM -> shared memory; then every warp: the sum over the
-//              cluster's pairs and the epilogue, a row a warp
+//   warps 2-17 TMEM -> shared memory; then every warp: the sum over the
+//              cluster's pairs and the epilogue, a row a warp (8 warps: 256 rows
+//              x 4096 x 512 9.1 us, 16 8.5)
 // ---------------------------------------------------------------------
-constexpr int kThreadsMid = 320;
+constexpr int kDrainMid = 16;      // warps that empty the accumulators
+constexpr int kThreadsMid = 64 + 32 * kDrainMid;
 constexpr int kMidRows = 1024;      // rows up to which this form is considered
 constexpr int kMidUnits = 40;       // units of a pass: 1024 rows / 64, and two ends a segment
 
@@ -1022,6 +1020,7 @@ struct MidUnit {
 struct MidParams {
   int N, n_kblk;
   int sf_blk_expert;
+  bool units_first;   // the units of a weight tile run side by side
   void* y;
   const bf16* resid;
   const bf16* bias;
@@ -1055,8 +1054,9 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
   const uint32_t cta = cluster_ctarank(), rank = cta & 1, lead_cta = cta & ~1u;
   const uint16_t both = (uint16_t)(3u << lead_cta);
   const int split = (int)gridDim.x >> 1, part_k = (int)(cta >> 1);   // the cluster is the x axis
-  const int blk = (int)blockIdx.y * 2 + (int)rank;   // this CTA's 128 output columns
-  const MidUnit u = p.unit[blockIdx.z];
+  // this CTA's 128 output columns, and its rows
+  const int blk = (int)(p.units_first ? blockIdx.z : blockIdx.y) * 2 + (int)rank;
+  const MidUnit u = p.unit[p.units_first ? blockIdx.y : blockIdx.z];
   const int nr = (u.hi + 31) & ~31;                  // rows the MMAs take
   const int xr = ((nr >> 1) + 31) & ~31;             // rows a CTA loads, in boxes of 32
   // this CTA's stages of the tile, and their first k-block
@@ -1190,15 +1190,15 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
   bool ok = true;
   if (w >= 2) {
     if constexpr (EPI == kEpiResid)
-      prefetch_resid(p, u.m0 + u.lo + part_k, split, u.m0 + u.hi, 256, (int)threadIdx.x - 64,
-                     blk * 128, 128);
+      prefetch_resid(p, u.m0 + u.lo + part_k, split, u.m0 + u.hi, 32 * kDrainMid,
+                     (int)threadIdx.x - 64, blk * 128, 128);
     // every MMA of the pair has completed, and with them every load of both CTAs
     ok = warp_wait(accf, 0, p.err, kDevWaitAccFull);
     tc_fence_after();
     const int wq = (int)(w & 3), n = wq * 32 + (int)lane_id();
     const uint32_t tb = tmem + ((uint32_t)(wq * 32) << 16);
 #pragma unroll 1
-    for (int c = (u.lo & ~15) + ((int)(w - 2) >> 2) * 16; c < u.hi && ok; c += 32) {
+    for (int c = (u.lo & ~15) + ((int)(w - 2) >> 2) * 16; c < u.hi && ok; c += 4 * kDrainMid) {
 #pragma unroll
       for (int h = 0; h < NA; ++h) {
         uint32_t r[16];
@@ -1216,8 +1216,7 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
   const int ncols = GU ? p.N / 2 : p.N, col = blk * 128 + (int)lane_id() * 4;
   if (ok && blk * 128 < ncols) {   // the last pair's second CTA may be past the columns
     constexpr int kWarps = kThreadsMid / 32;
-    const float4* mine = reinterpret_cast<const float4*>(part) + lane_id();
-    const uint32_t own = smem_u32(mine);
+    const uint32_t own = smem_u32(part) + lane_id() * 16;
     const int step = kWarps * split;
     auto finish = [&](auto r_, auto q_) {
       constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
@@ -1235,10 +1234,7 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
             for (int i = 0; i < R; ++i)
               if (j0 + i * step < u.hi) {
                 const int at = h * C::kRows + j0 + i * step;
-                if constexpr (Q == 1)
-                  v[q][h][i] = mine[at * 32];
-                else
-                  v[q][h][i] = ld_cluster4(from + at * 512);
+                v[q][h][i] = Q == 1 ? ld_shared4(own + at * 512) : ld_cluster4(from + at * 512);
               }
         }
         float4 t[NA][R];
@@ -1271,7 +1267,7 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
     };
     using std::integral_constant;
     if (split == 1)
-      finish(integral_constant<int, 8 / NA>{}, integral_constant<int, 1>{});
+      finish(integral_constant<int, 4 / NA>{}, integral_constant<int, 1>{});
     else if (split == 2)
       finish(integral_constant<int, 4 / NA>{}, integral_constant<int, 2>{});
     else
@@ -1577,6 +1573,7 @@ const int* mid_resident(int num_sms)
 
 struct MidPlan {
   int height = 64, split = 1;   // rows of a unit, pairs a tile
+  bool units_first = false;
   long ns = -1;
 };
 
@@ -1618,7 +1615,7 @@ inline long mid_kblk_ns(int nr, int ctas)
 template <bool GU>
 inline long mid_unit_ns(int nr)
 {
-  return GU ? 2800 + 44 * nr : 2700 + 21 * nr;
+  return GU ? 2800 + 38 * nr : 2700 + 18 * nr;
 }
 
 template <int EPI>
@@ -1649,6 +1646,11 @@ MidPlan mid_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* residen
       if (best.ns < 0 || ns < best.ns) {
         best.height = h;
         best.split = s;
+        // A weight tile's units side by side read it from HBM once; one after the
+        // other, tallest first, a short last round holds small ones only (two
+        // segments, 333 x 24576 x 4096 SwiGLU, 144 tiles on 74 places: 53.5 and 58
+        // us; 1000 x 4096 x 12288, 80 tiles: 64 and 52)
+        best.units_first = 2 * ((all - 1) % places + 1) > places;
         best.ns = ns;
       }
     }
@@ -1670,7 +1672,8 @@ int launch_mid(const GemmFp8Args& a, const SegInfo& seg, const MidPlan& plan, cu
   p.bias = static_cast<const bf16*>(a.bias);
   p.sy = a.sy;
   p.err = a.dev_err;
-  const int units = mid_units(seg, plan.height, p.unit);
+  p.units_first = plan.units_first;
+  const int units = mid_units(seg, plan.height, p.unit), tiles = mid_tiles<EPI>(a);
   CUtensorMap mx, mw, msx, msw;
   const uint64_t groups = fp8_groups(a.K);
   if (make_tma_2d(&mx, a.xq, a.M, a.K, 32, 1, err) ||
@@ -1680,7 +1683,8 @@ int launch_mid(const GemmFp8Args& a, const SegInfo& seg, const MidPlan& plan, cu
     return 2;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreadsMid);
-  cfg.gridDim = dim3(2 * plan.split, mid_tiles<EPI>(a), units);
+  cfg.gridDim = p.units_first ? dim3(2 * plan.split, units, tiles)
+                              : dim3(2 * plan.split, tiles, units);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attrs[2] = {};
