@@ -854,22 +854,10 @@ struct MapKeyHash {
 }  // namespace
 
 // A 2-D [rows][cols] row-major tensor (elsize 2 = bf16, 1 = int8), box of
-// 128 bytes x box_rows, 128-byte swizzle, zero fill out of bounds. Cached:
-// encoding costs microseconds and a layer calls the same maps every pass.
-int make_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint32_t box_rows,
-             int elsize, std::string* err)
+// 128 bytes x box_rows, 128-byte swizzle, zero fill out of bounds.
+int encode_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols,
+                  uint32_t box_rows, int elsize, std::string* err)
 {
-  static std::mutex mu;
-  static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-  const MapKey key{ptr, rows, cols, box_rows, elsize};
-  {
-    std::lock_guard<std::mutex> g(mu);
-    auto it = cache.find(key);
-    if (it != cache.end()) {
-      *out = it->second;
-      return 0;
-    }
-  }
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) {
     *err = "cuTensorMapEncodeTiled is unavailable (driver too old?)";
@@ -884,10 +872,28 @@ int make_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols,
          const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    *err = "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
-    return 1;
+  if (r == CUDA_SUCCESS) return 0;
+  *err = "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
+  return 1;
+}
+
+// The same, cached: encoding costs microseconds and a layer calls the same
+// maps every pass.
+int make_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                int elsize, std::string* err)
+{
+  static std::mutex mu;
+  static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
+  const MapKey key{ptr, rows, cols, box_rows, elsize};
+  {
+    std::lock_guard<std::mutex> g(mu);
+    auto it = cache.find(key);
+    if (it != cache.end()) {
+      *out = it->second;
+      return 0;
+    }
   }
+  if (encode_tma_2d(out, ptr, rows, cols, box_rows, elsize, err)) return 1;
   std::lock_guard<std::mutex> g(mu);
   if (cache.size() > 4096) cache.clear();
   cache.emplace(key, *out);

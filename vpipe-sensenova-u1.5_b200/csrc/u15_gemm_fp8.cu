@@ -879,7 +879,8 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   bool ok = true;
   if (w >= 2) {
     if constexpr (EPI == kEpiResid)
-      prefetch_resid(p, m0 + lo + rank, split, m0 + hi, 128, (int)threadIdx.x - 64, tile * 128, 128);
+      prefetch_resid(p, m0 + lo + rank, split, m0 + hi, 128, (int)threadIdx.x - 64, tile * 128,
+                     128);
     // every MMA of this CTA has completed, and with them every load
     ok = warp_wait(accf, 0, p.err, kDevWaitAccFull);
     tc_fence_after();
@@ -1366,9 +1367,9 @@ int launch_pair(const GemmFp8Args& a, const SegInfo& seg, int split, cudaStream_
   CUtensorMap ma, mb, mbh, msa, msb, msbh;
   const uint64_t wrows = (uint64_t)a.N * a.n_experts, groups = fp8_groups(a.K),
                  wblks = (uint64_t)p.sf_blk_expert * a.n_experts, xblks = (a.M + 127) / 128;
-  if (make_tma_2d(&ma, a.xq, a.M, a.K, 128, 1, err) ||
-      make_tma_2d(&mb, a.wq, wrows, a.K, 128, 1, err) ||
-      make_tma_2d(&mbh, a.wq, wrows, a.K, 64, 1, err) ||
+  if (encode_tma_2d(&ma, a.xq, a.M, a.K, 128, 1, err) ||
+      encode_tma_2d(&mb, a.wq, wrows, a.K, 128, 1, err) ||
+      encode_tma_2d(&mbh, a.wq, wrows, a.K, 64, 1, err) ||
       make_tma_fp8_scales(&msa, a.sx, xblks, groups, 2, err) ||
       make_tma_fp8_scales(&msb, a.sw, wblks, groups, 2, err) ||
       make_tma_fp8_scales(&msbh, a.sw, wblks, groups, 1, err))
@@ -1512,8 +1513,8 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cu
   const int tiles = few_tiles<EPI>(a);
   CUtensorMap mx, mw, msx, msw;
   const uint64_t groups = fp8_groups(a.K);
-  if (make_tma_2d(&mx, a.xq, a.M, a.K, MT, 1, err) ||
-      make_tma_2d(&mw, a.wq, (uint64_t)a.N * a.n_experts, a.K, 128, 1, err) ||
+  if (encode_tma_2d(&mx, a.xq, a.M, a.K, MT, 1, err) ||
+      encode_tma_2d(&mw, a.wq, (uint64_t)a.N * a.n_experts, a.K, 128, 1, err) ||
       make_tma_fp8_scales(&msx, a.sx, (a.M + 127) / 128, groups, 1, err) ||
       make_tma_fp8_scales(&msw, a.sw, (uint64_t)p.sf_blk_expert * a.n_experts, groups, 1, err))
     return 2;
@@ -1676,8 +1677,8 @@ int launch_mid(const GemmFp8Args& a, const SegInfo& seg, const MidPlan& plan, cu
   const int units = mid_units(seg, plan.height, p.unit), tiles = mid_tiles<EPI>(a);
   CUtensorMap mx, mw, msx, msw;
   const uint64_t groups = fp8_groups(a.K);
-  if (make_tma_2d(&mx, a.xq, a.M, a.K, 32, 1, err) ||
-      make_tma_2d(&mw, a.wq, (uint64_t)a.N * a.n_experts, a.K, 128, 1, err) ||
+  if (encode_tma_2d(&mx, a.xq, a.M, a.K, 32, 1, err) ||
+      encode_tma_2d(&mw, a.wq, (uint64_t)a.N * a.n_experts, a.K, 128, 1, err) ||
       make_tma_fp8_scales(&msx, a.sx, (a.M + 127) / 128, groups, 1, err) ||
       make_tma_fp8_scales(&msw, a.sw, (uint64_t)p.sf_blk_expert * a.n_experts, groups, 1, err))
     return 2;

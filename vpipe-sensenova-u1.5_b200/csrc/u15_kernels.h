@@ -222,8 +222,11 @@ int attention_tc(const TcAttnArgs& a, cudaStream_t st, std::string* err);
 // rest to the mma.sync kernel.
 bool attention_tc_serves(int mode, int tk, const int32_t* t_index);
 
-// A cached 2-D TMA map over a row-major [rows][cols] tensor (elsize 2 = bf16,
-// 1 = int8): box of 128 bytes x box_rows, 128-byte swizzle, zero fill.
+// A 2-D TMA map over a row-major [rows][cols] tensor (elsize 2 = bf16, 1 =
+// int8 or e4m3): box of 128 bytes x box_rows, 128-byte swizzle, zero fill.
+int encode_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols,
+                  uint32_t box_rows, int elsize, std::string* err);
+// The same, cached.
 int make_tma_2d(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols,
                 uint32_t box_rows, int elsize, std::string* err);
 
