@@ -35,8 +35,8 @@ using bf16 = __nv_bfloat16;
 // SPLIT: fewer tiles than pairs. The k-blocks of a tile are split over the
 // pairs of a cluster of 4, 6 or 8 CTAs, a cluster a tile; each CTA leaves its
 // 128 x 256 partial sums in shared memory, over the ring, and finishes its share
-// of the rows from every pair's (in pair order): 512 rows x 4096 x 12288 are
-// 32 tiles, 37 us on 32 pairs.
+// of the rows from every pair's (in pair order): 1100 rows x 1024 x 12288 are
+// 20 tiles, 25 us on 60 pairs.
 // ---------------------------------------------------------------------
 constexpr int kKps = 2;                        // k-blocks per stage
 constexpr int kStg = 3;
@@ -983,14 +983,20 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
 // segment has there rounded up to 32, half of them loaded by each CTA. A
 // CTA's accumulator then is its own 128 columns of all the unit's rows, and
 // the epilogue is the few-row form's. The k-blocks of a tile are split over the
-// pairs of a cluster.
+// pairs of a cluster. A stage is as large as the unit's rows make it, so small units
+// have more of them in flight.
+//   A k-block of 256 rows takes 286 ns, the MMAs' own time 270; of 64 rows 160, the
+// weights' loads 135 at 64 bytes a cycle. One k-block a stage took 50 to 130 ns more
+// (the handshake of two CTAs costs ~200 a stage). What a tile spends outside its
+// k-blocks, 4 to 8.5 us, no other tile on its SM hides: the ring and the partial
+// sums take the shared memory of one CTA.
 //   warp 0     TMA producer (both CTAs)
 //   warp 1     MMA issuer (leader)
-//   warps 2-17 TMEM -> shared memory; then every warp: the sum over the
-//              cluster's pairs and the epilogue, a row a warp (8 warps: 256 rows
-//              x 4096 x 512 9.1 us, 16 8.5)
+//   warps 2-17 TMEM -> shared memory (an unsplit SwiGLU tile: with SwiGLU done); then
+//              every warp: the sum over the cluster's pairs and the epilogue, a row
+//              a warp (8 warps: 256 rows x 4096 x 512 9.1 us, 16 8.5)
 // ---------------------------------------------------------------------
-constexpr int kDrainMid = 16;      // warps that empty the accumulators
+constexpr int kDrainMid = 16;       // warps that empty the accumulators
 constexpr int kThreadsMid = 64 + 32 * kDrainMid;
 constexpr int kMidRows = 1024;      // rows up to which this form is considered
 constexpr int kMidUnits = 40;       // units of a pass: 1024 rows / 64, and two ends a segment
@@ -1200,14 +1206,20 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
     const uint32_t tb = tmem + ((uint32_t)(wq * 32) << 16);
 #pragma unroll 1
     for (int c = (u.lo & ~15) + ((int)(w - 2) >> 2) * 16; c < u.hi && ok; c += 4 * kDrainMid) {
+      uint32_t r[NA][16];
 #pragma unroll
-      for (int h = 0; h < NA; ++h) {
-        uint32_t r[16];
-        tmem_ld16(tb + h * C::kRows + c, r);
-        tmem_ld_wait();
+      for (int h = 0; h < NA; ++h) tmem_ld16(tb + h * C::kRows + c, r[h]);
+      tmem_ld_wait();
+      float* const to = part + c * 128 + n;
+      if (GU && split == 1) {   // gate and up of a column are here together
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          part[(h * C::kRows + c + i) * 128 + n] = __uint_as_float(r[i]);
+          to[i * 128] = swiglu1(__uint_as_float(r[0][i]), __uint_as_float(r[NA - 1][i]));
+      } else {
+#pragma unroll
+        for (int h = 0; h < NA; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) to[(h * C::kRows + i) * 128] = __uint_as_float(r[h][i]);
       }
     }
   }
@@ -1221,16 +1233,17 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
     const int step = kWarps * split;
     auto finish = [&](auto r_, auto q_) {
       constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
+      constexpr int NS = Q == 1 ? 1 : NA;   // sums a column: SwiGLU of an unsplit tile is done
       for (int j0 = u.lo + part_k + (int)w * split; j0 < u.hi; j0 += R * step) {
         uint2 a[R] = {};
         addend4<EPI>(a, p, u.m0 + j0, step, (u.hi - j0 + step - 1) / step, u.expert, col, ncols);
-        float4 v[Q][NA][R] = {};
+        float4 v[Q][NS][R] = {};
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
           if (q >= split) break;
           const uint32_t from = mapa_shared(own, 2 * q + rank);
 #pragma unroll
-          for (int h = 0; h < NA; ++h)
+          for (int h = 0; h < NS; ++h)
 #pragma unroll
             for (int i = 0; i < R; ++i)
               if (j0 + i * step < u.hi) {
@@ -1238,9 +1251,9 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
                 v[q][h][i] = Q == 1 ? ld_shared4(own + at * 512) : ld_cluster4(from + at * 512);
               }
         }
-        float4 t[NA][R];
+        float4 t[NS][R];
 #pragma unroll
-        for (int h = 0; h < NA; ++h)
+        for (int h = 0; h < NS; ++h)
 #pragma unroll
           for (int i = 0; i < R; ++i) {
             t[h][i] = v[0][h][i];
@@ -1256,7 +1269,7 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
         for (int i = 0; i < R; ++i) {
           if (j0 + i * step >= u.hi) break;
           float o[4] = {t[0][i].x, t[0][i].y, t[0][i].z, t[0][i].w};
-          if constexpr (GU) {
+          if constexpr (NS == 2) {
             o[0] = swiglu1(o[0], t[1][i].x);
             o[1] = swiglu1(o[1], t[1][i].y);
             o[2] = swiglu1(o[2], t[1][i].z);
@@ -1268,7 +1281,7 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
     };
     using std::integral_constant;
     if (split == 1)
-      finish(integral_constant<int, 4 / NA>{}, integral_constant<int, 1>{});
+      finish(integral_constant<int, 4>{}, integral_constant<int, 1>{});
     else if (split == 2)
       finish(integral_constant<int, 4 / NA>{}, integral_constant<int, 2>{});
     else
@@ -1601,9 +1614,9 @@ int mid_tiles(const GemmFp8Args& a)
 }
 
 // Nanoseconds of a k-block of a unit of nr rows, and of its set-up, first loads and
-// epilogue, as measured (4096 columns of one unit, K 512 to 12288: 64 rows 4.7 to
-// 19.7 us, 128 6.0 to 22.5, 256 9.3 to 35.8; the SwiGLU form's two accumulators, K
-// 512 and 2048: 128 rows 9.7 and 13.6, 192 13.1 and 18.8).
+// epilogue, as measured (4096 columns of one unit, K 512 and 4096: 64 rows 4.5 and
+// 9.3 us, 128 5.7 and 10.7, 256 8.5 and 16.6; the SwiGLU form, two units of 192 rows x
+// 16384: 10.7 and 24.3).
 // With many CTAs at it the SwiGLU form's loads count (two weight tiles a k-block):
 // 12.3 TB/s into all of the chip's shared memory.
 template <bool GU>
@@ -1616,7 +1629,7 @@ inline long mid_kblk_ns(int nr, int ctas)
 template <bool GU>
 inline long mid_unit_ns(int nr)
 {
-  return GU ? 2800 + 38 * nr : 2700 + 18 * nr;
+  return GU ? 2800 + 32 * nr : 2700 + 18 * nr;
 }
 
 template <int EPI>
