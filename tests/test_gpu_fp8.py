@@ -255,7 +255,7 @@ def test_linear_empty_and_single_row_segments(ops):
 
 def test_linear_unaligned_outputs(ops):
     """y, residual and bias off every 16-byte boundary."""
-    for M, N in [(5, 256), (70, 512), (300, 512)]:
+    for M, N in [(5, 256), (70, 512), (300, 512), (1100, 512)]:
         K, E = 256, 1
         xq, xs = quantised(M, K, 15)
         W, wq, ws = weights(E, N, K, 16)
@@ -421,7 +421,10 @@ EIGHT = [(0, 63, 0), (63, 64, 1), (64, 65, 0), (65, 161, 1), (161, 257, 0), (257
     (160, 640, 136, [(0, 64, 0), (64, 160, 1)]), (193, 4240, 256, [(0, 127, 1), (127, 193, 0)]),
     (257, 8208, 392, None), (320, 2176, 260, [(0, 1, 1), (1, 320, 0)]),
     (1000, 528, 768, [(0, 77, 0), (77, 1000, 1)]), (1024, 272, 1160, EIGHT), (1024, 1296, 513, None),
-    (1025, 1296, 513, None)])
+    (1025, 1296, 513, None),
+    # more rows, of columns that leave them off 32 bytes or end inside a run of 32
+    (1100, 144, 1000, [(0, 300, 1), (300, 1100, 0)]), (1301, 272, 777, [(0, 33, 0), (33, 1301, 1)]),
+    (1200, 144, 272, None)])
 @pytest.mark.parametrize("epi", [STORE, RESID, F32])
 def test_linear_units(ops, M, K, N, segs, epi):
     run_linear(ops, M, K, N, segs, epi, bias=epi != RESID)
@@ -472,6 +475,19 @@ def test_swiglu(ops, M, K, I, segs):
     # the error before rounding also moves the step: half a step at |want| + err
     v = F.values(q[:M * I].reshape(M, I), sb)
     assert (np.abs(v - want) <= F.half_step(np.abs(want) + err, sb) + err).all()
+
+
+@pytest.mark.parametrize("M", [20, 200, 1100])
+def test_swiglu_unaligned_output(ops, M):
+    K, I = 256, 384
+    xq, xs = quantised(M, K, 71)
+    W, wq, ws = weights(1, 2 * I, K, 72)
+    args = (dev_u8(xq), dev_u8(F.pack(xs, K)), wq, ws, None)
+    want = torch.empty(M * I, dtype=torch.bfloat16, device="cuda")
+    ops.mot_linear_fp8(*args, want, M, K, 2 * I, epilogue=SWIGLU)
+    y = torch.full((M * I + 2,), 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.mot_linear_fp8(*args, y[1:], M, K, 2 * I, epilogue=SWIGLU)
+    assert torch.equal(y[1:-1], want) and y[0] == 5 and y[-1] == 5
 
 
 # ------------------------------------------------------------------ together

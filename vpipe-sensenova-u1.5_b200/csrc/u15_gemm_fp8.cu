@@ -42,7 +42,9 @@ constexpr int kKps = 2;                        // k-blocks per stage
 constexpr int kStg = 3;
 constexpr int kTileBytes = 128 * 128;          // one operand, one k-block, one CTA
 constexpr int kStageBytes = 2 * kKps * kTileBytes + 2048;   // operands, then the scales
-constexpr int kSmemPair = kStg * kStageBytes + 1024 /*align*/ + 2048 /*amax*/ + 256 /*bars*/;
+constexpr int kTurn = 32 * 17;                 // floats a warp turns rows in (turned32)
+constexpr int kSmemPair =
+    kStg * kStageBytes + 1024 /*align*/ + 2048 /*amax*/ + 256 /*bars*/ + 8 * kTurn * 4;
 constexpr int kThreadsPair = 320;
 constexpr int kMaxPairs = 4;   // pairs a tile: clusters of 8 CTAs, the portable size
 constexpr int kAccStep = 224;                  // accumulator 1 starts 32 columns early
@@ -102,57 +104,91 @@ __device__ __forceinline__ float swiglu1(float g, float u)
   return __fdividef(g, 1.0f + expf(-g)) * u;
 }
 
-// 32 columns of one row; columns >= ncols dropped
-__device__ __forceinline__ void store32(bf16* dst, const float (&v)[32], int col0, int ncols)
+// 32 columns of one row, 32-byte aligned
+__device__ __forceinline__ void store32(bf16* dst, const float (&v)[32])
 {
-  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint32_t o[8];
+  for (int q = 0; q < 2; ++q) {
+    uint32_t o[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = pack_bf2(v[q * 16 + 2 * i], v[q * 16 + 2 * i + 1]);
-      store32b(dst + q * 16, o);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (col0 + i < ncols) dst[i] = f2bf(v[i]);
+    for (int i = 0; i < 8; ++i) o[i] = pack_bf2(v[q * 16 + 2 * i], v[q * 16 + 2 * i + 1]);
+    store32b(dst + q * 16, o);
   }
 }
-__device__ __forceinline__ void store32(float* dst, const float (&v)[32], int col0, int ncols)
+__device__ __forceinline__ void store32(float* dst, const float (&v)[32])
 {
-  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint32_t o[8];
+  for (int q = 0; q < 4; ++q) {
+    uint32_t o[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(v[q * 8 + i]);
-      store32b(dst + q * 8, o);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (col0 + i < ncols) dst[i] = v[i];
+    for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(v[q * 8 + i]);
+    store32b(dst + q * 8, o);
   }
 }
-__device__ __forceinline__ void add32(float (&v)[32], const bf16* src, int col0, int ncols)
+__device__ __forceinline__ void add32(float (&v)[32], const bf16* src)
 {
-  if (col0 + 32 <= ncols && (reinterpret_cast<uintptr_t>(src) & 31) == 0) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint32_t u[8];
-      load32b(src + q * 16, u);
+  for (int q = 0; q < 2; ++q) {
+    uint32_t u[8];
+    load32b(src + q * 16, u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 a = unpack_bf2(u[i]);
-        v[q * 16 + 2 * i] += a.x;
-        v[q * 16 + 2 * i + 1] += a.y;
+    for (int i = 0; i < 8; ++i) {
+      const float2 a = unpack_bf2(u[i]);
+      v[q * 16 + 2 * i] += a.x;
+      v[q * 16 + 2 * i + 1] += a.y;
+    }
+  }
+}
+// Whether every row of [rows][cols] values of `size` bytes begins on 32 bytes.
+__device__ __forceinline__ bool rows_lined(const void* p, long cols, int size)
+{
+  return (reinterpret_cast<uintptr_t>(p) & 31) == 0 && (cols * size & 31) == 0;
+}
+// 32 rows of 32 columns of a warp, a row a lane, where rows do not begin on 32 bytes or
+// the columns end: turned in shared memory, so that 16 lanes store (and read the
+// residual of) 16 neighbouring columns. With each lane at its own row an
+// instruction touched 32 sectors for 64 bytes: 3282 rows x 2043 x 336 75 and 18.5 us.
+template <int EPI, class T, class P>
+__device__ __forceinline__ void turned32(const P& p, float* turn, const float (&v)[32], int row0,
+                                         int row_lo, int row_hi, int expert, int col0, int ncols)
+{
+  const int lane = (int)lane_id(), r = lane >> 4, c = lane & 15;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int col = col0 + h * 16 + c;
+    if (col0 + h * 16 >= ncols) break;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = v[h * 16 + j];
+    __syncwarp();
+    const bool here = col < ncols;
+    float b = 0.0f;
+    if ((EPI == kEpiStore || EPI == kEpiStoreF32) && p.bias != nullptr && here)
+      b = bf2f(p.bias[(long)expert * p.N + col]);
+    float x[16], a[16] = {};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = turn[(2 * i + r) * 17 + c];
+    if constexpr (EPI == kEpiResid) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int row = row0 + 2 * i + r;
+        if (here && row >= row_lo && row < row_hi) a[i] = bf2f(p.resid[(long)row * ncols + col]);
       }
     }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (col0 + i < ncols) v[i] += bf2f(src[i]);
+    for (int i = 0; i < 16; ++i) {
+      const int row = row0 + 2 * i + r;
+      if (!here || row < row_lo || row >= row_hi) continue;
+      if (EPI == kEpiResid)
+        x[i] += a[i];
+      else if (p.bias != nullptr)
+        x[i] += b;
+      T* const y = static_cast<T*>(p.y) + (long)row * ncols + col;
+      if constexpr (sizeof(T) == 4)
+        *y = x[i];
+      else
+        *y = f2bf(x[i]);
+    }
   }
 }
 
@@ -444,6 +480,7 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
     // ---------------- epilogue (warps 2..9, both CTAs) ----------------
     const int wq = (int)(w & 3), wh = (int)(w - 2) >> 2;   // lane quadrant, half of the columns
     const int r_in = wq * 32 + (int)lane_id();
+    float* const turn = reinterpret_cast<float*>(bars) + 64 + ((int)w - 2) * kTurn;
     const uint32_t accr_leader = mapa_shared(accr, lead_cta);
     int lt = 0;
     for (int t = pair; t < n_tiles; t += n_pairs, ++lt) {
@@ -486,10 +523,14 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
         }
         if constexpr (EPI == kEpiSwiglu) {
           bf16* yrow = static_cast<bf16*>(p.y) + (long)row * nout + ti.nb * 128;
-          if (row_ok) {
+          const bool lined = rows_lined(p.y, nout, 2);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              store32(yrow + run[i] * 32, h[i], ti.nb * 128 + run[i] * 32, nout);
+          for (int i = 0; i < 2; ++i) {
+            if (!lined)
+              turned32<EPI, bf16>(p, turn, h[i], row - (int)lane_id(), ti.row_lo, ti.row_hi,
+                                  ti.expert, ti.nb * 128 + run[i] * 32, nout);
+            else if (row_ok)
+              store32(yrow + run[i] * 32, h[i]);
           }
         } else {
           // the row's largest of 128 outputs, over the quadrant's two warps
@@ -532,6 +573,10 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           }
         }
       } else {
+        using Out = std::conditional_t<EPI == kEpiStoreF32, float, bf16>;
+        const bool lined = rows_lined(p.y, p.N, sizeof(Out)) &&
+                           (EPI == kEpiResid ? rows_lined(p.resid, p.N, 2)
+                                             : p.bias == nullptr || rows_lined(p.bias, p.N, 2));
         const int n0 = ti.nb * 256 + (half ? 128 * ti.half : 0);
         const int nch = half ? 2 : 4;                 // chunks of 32 columns of this warp
         const int first = half ? wh * 2 : wh * 4;
@@ -547,16 +592,19 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
           tmem_ld_wait();
           release();
           const int col0 = n0 + c * 32;
-          if (!row_ok || col0 >= p.N) continue;
+          if (col0 >= p.N) continue;
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          if (p.bias != nullptr) add32(v, p.bias + (long)ti.expert * p.N + col0, col0, p.N);
-          if constexpr (EPI == kEpiResid) add32(v, p.resid + (long)row * p.N + col0, col0, p.N);
-          if constexpr (EPI == kEpiStoreF32)
-            store32(static_cast<float*>(p.y) + (long)row * p.N + col0, v, col0, p.N);
-          else
-            store32(static_cast<bf16*>(p.y) + (long)row * p.N + col0, v, col0, p.N);
+          if (!lined || col0 + 32 > p.N) {
+            turned32<EPI, Out>(p, turn, v, row - (int)lane_id(), ti.row_lo, ti.row_hi, ti.expert,
+                               col0, p.N);
+          } else if (row_ok) {
+            if (EPI != kEpiResid && p.bias != nullptr)
+              add32(v, p.bias + (long)ti.expert * p.N + col0);
+            if constexpr (EPI == kEpiResid) add32(v, p.resid + (long)row * p.N + col0);
+            store32(static_cast<Out*>(p.y) + (long)row * p.N + col0, v);
+          }
         }
       }
     }
