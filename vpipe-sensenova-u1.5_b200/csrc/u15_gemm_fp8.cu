@@ -165,22 +165,25 @@ __device__ __forceinline__ void turned32(const P& p, float* turn, const float (&
     float b = 0.0f;
     if ((EPI == kEpiStore || EPI == kEpiStoreF32) && p.bias != nullptr && here)
       b = bf2f(p.bias[(long)expert * p.N + col]);
-    float x[16], a[16] = {};
+    // the residual's bits, all loads in flight together: places that are not the
+    // segment's read one that is
+    uint32_t a[16] = {};
+    if constexpr (EPI == kEpiResid) {
+      const unsigned short* src =
+          reinterpret_cast<const unsigned short*>(p.resid) + min(col, ncols - 1);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        a[i] = src[(long)min(max(row0 + 2 * i + r, row_lo), row_hi - 1) * ncols];
+    }
+    float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = turn[(2 * i + r) * 17 + c];
-    if constexpr (EPI == kEpiResid) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int row = row0 + 2 * i + r;
-        if (here && row >= row_lo && row < row_hi) a[i] = bf2f(p.resid[(long)row * ncols + col]);
-      }
-    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int row = row0 + 2 * i + r;
       if (!here || row < row_lo || row >= row_hi) continue;
       if (EPI == kEpiResid)
-        x[i] += a[i];
+        x[i] += __uint_as_float(a[i] << 16);
       else if (p.bias != nullptr)
         x[i] += b;
       T* const y = static_cast<T*>(p.y) + (long)row * ncols + col;
@@ -238,15 +241,17 @@ __device__ __forceinline__ void addend4(uint2 (&a)[R], const P& p, long row, int
       for (int i = 0; i < R; ++i)
         if (i < n_rows) a[i] = *reinterpret_cast<const uint2*>(src + i * pitch);
     } else {
+      // places past the columns or the rows read the last there is
       const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
+      uint32_t x[R][4];
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        uint32_t x[4] = {};
+      for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (i < n_rows && col + k < ncols) x[k] = u[i * pitch + k];
-        a[i] = make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
-      }
+          x[i][k] = u[min(i, n_rows - 1) * pitch + min(k, ncols - 1 - col)];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        a[i] = make_uint2(x[i][0] | x[i][1] << 16, x[i][2] | x[i][3] << 16);
     }
   }
 }
