@@ -255,7 +255,7 @@ def test_linear_empty_and_single_row_segments(ops):
 
 def test_linear_unaligned_outputs(ops):
     """y, residual and bias off every 16-byte boundary."""
-    for M, N in [(5, 256), (70, 512), (300, 512), (1100, 512)]:
+    for M, N in [(5, 256), (70, 512), (300, 512), (2100, 512)]:
         K, E = 256, 1
         xq, xs = quantised(M, K, 15)
         W, wq, ws = weights(E, N, K, 16)
@@ -378,7 +378,9 @@ def random_quantised(ops, rows, cols, seed, std):
     (512, 2064, 4096, [(0, 512, 0)]), (300, 12288, 2048, [(0, 300, 1)]),
     (400, 8192, 1536, [(0, 100, 0), (100, 400, 1)]), (450, 2304, 4000, [(0, 130, 1), (130, 450, 0)]),
     (1100, 12288, 1024, [(0, 1100, 0)]), (1030, 2320, 1500, [(0, 70, 1), (70, 1030, 0)]),
-    (1300, 4096, 520, [(0, 700, 1), (700, 700, 0), (700, 1300, 0)])])
+    (1300, 4096, 520, [(0, 700, 1), (700, 700, 0), (700, 1300, 0)]),
+    (2100, 4096, 512, [(0, 2100, 1)]), (2200, 2320, 700, [(0, 70, 1), (70, 2200, 0)]),
+    (2500, 1168, 256, [(0, 700, 1), (700, 700, 0), (700, 2500, 0)])])
 @pytest.mark.parametrize("epi", [STORE, RESID, SWIGLU])
 def test_many_tiles(ops, M, K, N, segs, epi):
     """More tiles than CTA pairs: the accumulators' shared columns, the scale
@@ -424,7 +426,8 @@ EIGHT = [(0, 63, 0), (63, 64, 1), (64, 65, 0), (65, 161, 1), (161, 257, 0), (257
     (1025, 1296, 513, None),
     # more rows, of columns that leave them off 32 bytes or end inside a run of 32
     (1100, 144, 1000, [(0, 300, 1), (300, 1100, 0)]), (1301, 272, 777, [(0, 33, 0), (33, 1301, 1)]),
-    (1200, 144, 272, None)])
+    (1200, 144, 272, None), (2100, 144, 1000, [(0, 300, 1), (300, 2100, 0)]),
+    (2201, 272, 777, [(0, 33, 0), (33, 2201, 1)]), (2048, 144, 272, None), (2049, 16, 272, None)])
 @pytest.mark.parametrize("epi", [STORE, RESID, F32])
 def test_linear_units(ops, M, K, N, segs, epi):
     run_linear(ops, M, K, N, segs, epi, bias=epi != RESID)
@@ -477,7 +480,7 @@ def test_swiglu(ops, M, K, I, segs):
     assert (np.abs(v - want) <= F.half_step(np.abs(want) + err, sb) + err).all()
 
 
-@pytest.mark.parametrize("M", [20, 200, 1100])
+@pytest.mark.parametrize("M", [20, 200, 2100])
 def test_swiglu_unaligned_output(ops, M):
     K, I = 256, 384
     xq, xs = quantised(M, K, 71)

@@ -1051,8 +1051,9 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
 // ---------------------------------------------------------------------
 constexpr int kDrainMid = 16;       // warps that empty the accumulators
 constexpr int kThreadsMid = 64 + 32 * kDrainMid;
-constexpr int kMidRows = 1024;      // rows up to which this form is considered
-constexpr int kMidUnits = 40;       // units of a pass: 1024 rows / 64, and two ends a segment
+constexpr int kMidRows = 2048;      // rows up to which this form is considered
+constexpr int kMidRounds = 1024;    // rows up to which in more than one round of tiles
+constexpr int kMidUnits = 48;       // units of a pass: 2048 rows / 64, and two ends a segment
 
 template <bool GU>
 struct MidCfg {
@@ -1641,6 +1642,7 @@ const int* mid_resident(int num_sms)
 struct MidPlan {
   int height = 64, split = 1;   // rows of a unit, pairs a tile
   bool units_first = false;
+  bool one_round = false;
   long ns = -1;
 };
 
@@ -1718,6 +1720,7 @@ MidPlan mid_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* residen
         // segments, 333 x 24576 x 4096 SwiGLU, 144 tiles on 74 places: 53.5 and 58
         // us; 1000 x 4096 x 12288, 80 tiles: 64 and 52)
         best.units_first = 2 * ((all - 1) % places + 1) > places;
+        best.one_round = all <= places;
         best.ns = ns;
       }
     }
@@ -1767,10 +1770,13 @@ int launch_mid(const GemmFp8Args& a, const SegInfo& seg, const MidPlan& plan, cu
                                                                                                : 2;
 }
 
-// More than 64 rows: tiles of 256 rows (pairs, one or several a tile), or up to 1024
+// More than 64 rows: tiles of 256 rows (pairs, one or several a tile), or up to 2048
 // rows units of the rows there are, whichever form takes less time by the models
 // above (333 rows in two segments x 4096 x 12288: 28 us, in tiles of 256 or
 // 128 rows 40; 1000 rows 52 and 62; 100 rows x 6144 x 4096: 13 to 16 and 16 to 21).
+// Above 1024 rows only where its tiles all run at once: their epilogues overlap
+// nothing, the persistent pairs' do (1512 rows x 1148 x 960 7.4 and 12.3 us, 1418 x
+// 4864 x 10592, two rounds, 79 and 67).
 template <int EPI>
 int launch_many(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::string* err)
 {
@@ -1803,7 +1809,8 @@ int launch_many(const GemmFp8Args& a, const SegInfo& seg, cudaStream_t st, std::
     const int* resident = mid_resident<EPI>(a.num_sms);
     if (resident == nullptr) return 2;
     const MidPlan mid = mid_plan_of<EPI>(a, seg, resident);
-    if (mid.ns < pair_ns) return launch_mid<EPI>(a, seg, mid, st, err);
+    if (mid.ns < pair_ns && (a.M <= kMidRounds || mid.one_round))
+      return launch_mid<EPI>(a, seg, mid, st, err);
   }
   return split > 1 ? launch_pair<EPI, true>(a, seg, split, st, err)
                    : launch_pair<EPI, false>(a, seg, 1, st, err);
