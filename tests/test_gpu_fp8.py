@@ -418,7 +418,8 @@ EIGHT = [(0, 63, 0), (63, 64, 1), (64, 65, 0), (65, 161, 1), (161, 257, 0), (257
 
 
 @pytest.mark.parametrize("M,K,N,segs", [
-    (65, 16, 128, None), (66, 272, 129, [(0, 65, 1), (65, 66, 0)]),
+    (65, 16, 128, None), (90, 656, 100, None), (130, 784, 128, [(0, 1, 0), (1, 130, 1)]),
+    (66, 272, 129, [(0, 65, 1), (65, 66, 0)]),
     (96, 400, 384, [(0, 32, 0), (32, 96, 1)]), (97, 1168, 640, [(0, 31, 1), (31, 97, 0)]),
     (160, 640, 136, [(0, 64, 0), (64, 160, 1)]), (193, 4240, 256, [(0, 127, 1), (127, 193, 0)]),
     (257, 8208, 392, None), (320, 2176, 260, [(0, 1, 1), (1, 320, 0)]),
@@ -567,7 +568,7 @@ def test_ffn_close_to_unquantised(ops):
 def test_other_stream_and_graph(ops):
     """On a side stream, and captured into a graph and replayed on new inputs;
     two graphs with workspaces of their own, replayed in turn."""
-    for rows in (3, 300):
+    for rows in (3, 300, 1500, 2100):
         h, i = 512, 256
         segs = segments_of(rows, "two")
         t = ffn_inputs(rows, h, i, 81)

@@ -1692,11 +1692,15 @@ MidPlan mid_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* residen
 {
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   const int n_kblk = fp8_blocks(a.K), tiles = mid_tiles<EPI>(a);
+  // every pair of a split tile has a stage: one without would add what its
+  // accumulators held
+  constexpr int kps = MidCfg<GU>::kKps;
+  const int most = std::min(kMaxPairs, (n_kblk + kps - 1) / kps);
   MidPlan best;
   for (int h = 64; h <= MidCfg<GU>::kRows; h += 64) {
     MidUnit unit[kMidUnits];
     const int n = mid_units(seg, h, unit);
-    for (int s = 1; s <= kMaxPairs && s <= n_kblk; ++s) {
+    for (int s = 1; s <= most; ++s) {
       // tile i's time, the tiles in order of their units' heights
       const long places = resident[s], all = (long)tiles * n;
       auto time = [&](long i) {
