@@ -241,7 +241,9 @@ int u15c_dequant_fp8(u15c_stream stream, const uint8_t* q, const uint8_t* scale,
  * pass: s = bf16(x + delta); q, scale = the quantised rows of
  * s * rsqrt(mean(s^2) + eps) * w_e. delta NULL: s = x. x_out, when non-NULL,
  * receives s (it may be x or delta). w_stack and segments as
- * u15c_mot_rms_norm. Feeds u15c_mot_linear_fp8 directly. */
+ * u15c_mot_rms_norm. The mean is an f32 sum: of a row that holds an Inf, or
+ * whose squares add up past f32 (one |s| of 1.85e19 does), the finite values
+ * become 0. Feeds u15c_mot_linear_fp8 directly. */
 int u15c_mot_add_rms_norm_quant_fp8(u15c_stream stream, const void* x, const void* delta,
                                     const void* w_stack, int n_experts, const int* seg_off,
                                     const int* seg_expert, int nseg, void* x_out, uint8_t* q,

@@ -76,10 +76,12 @@ __device__ __forceinline__ float rsqrt_newton(float v)
   const float e = __fmaf_rn(-l, r, __fmaf_rn(-h, r, 1.0f));
   return v == INFINITY ? 0.0f : __fmaf_rn(0.5f * r, e, r);
 }
-// acc / dim the same way: inv_dim = 1 / dim as a rounded value and its rest
+// acc / dim the same way: inv_dim = 1 / dim as a rounded value and its rest. A sum
+// past f32's range stays Inf (the rest, zero or negative for most widths, would
+// make it NaN), and the row's finite values become 0.
 __device__ __forceinline__ float mean_of(float acc, float2 inv_dim)
 {
-  return __fmaf_rn(acc, inv_dim.x, acc * inv_dim.y);
+  return acc < INFINITY ? __fmaf_rn(acc, inv_dim.x, acc * inv_dim.y) : acc;
 }
 
 constexpr int kNormSmem = 200 * 1024;   // bytes of row stages on an SM
