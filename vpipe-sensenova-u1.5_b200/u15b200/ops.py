@@ -28,8 +28,14 @@ def _stream():
     return _raw_stream(torch.cuda.current_device())
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_device = torch._C._cuda_getDevice   # the current device, for calls that hold CUDA tensors
+def _public_stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# torch's own bindings, where this build of it has them (one without CUDA does not)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
+# the current device, for calls that hold CUDA tensors
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 # array types, kept: making one takes longer than filling it
