@@ -610,7 +610,10 @@ int u15c_dequant_affine(u15c_stream stream, const uint32_t* codes, const void* s
  * gains N(norm_mean, norm_std). */
 int u15c_model_bind_random(u15c_model* m, u15c_stream stream, uint64_t seed, float std,
                            float norm_mean, float norm_std);
-/* Build the W8A8 twins (per-output-channel int8) from the bound bf16. */
+/* Build the W8A8 twins (per-output-channel int8) and the e4m3 twins (a scale
+ * per 128 x 128 block), whichever the model was created with, from the bound
+ * bf16. An fp8 pass is refused until it is called, and again after a bind of
+ * any projection (norms have no twins). */
 int u15c_model_finalize(u15c_model* m, u15c_stream stream);
 
 size_t u15c_model_weight_bytes(const u15c_model* m);
@@ -643,7 +646,8 @@ int u15c_kv_write(u15c_kv* kv, u15c_stream stream, int layer, int which_v, const
 
 #define U15C_FWD_INT8 1u /* W8A8 projections (i8_gemm) */
 #define U15C_FWD_SAGE 2u /* Sage int8-QK on the bidirectional pass */
-#define U15C_FWD_FP8 4u  /* e4m3 projections, a scale per block of 128 (not with _INT8) */
+#define U15C_FWD_FP8 4u  /* e4m3 projections, a scale per block of 128 (not with _INT8);
+                          * the twins must be of the weights bound now */
 
 /* The Sage tier's `dense_layers` (vpipe::genai::sage::Config, set through
  * MetalOps::set_sage, src/u15-metal-ops.cc:789-814, and honoured by

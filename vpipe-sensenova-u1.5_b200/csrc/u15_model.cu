@@ -143,6 +143,9 @@ struct u15c_model {
   int sage_dense_layers = 0;
   std::vector<LayerW> layers;
   bf16* final_norm = nullptr;   // [E][H]
+  // the e4m3 twins are of the projections bound now: set by finalize, cleared
+  // by whatever binds one of them
+  bool fp8_current = false;
   size_t weight_bytes = 0;
   std::vector<void*> allocs;
 
@@ -434,10 +437,6 @@ int layer_impl(u15c_model* m, cudaStream_t st, int li, bf16* x_all, int M,
   // (sdpa_steel's `sage_layer >= dense_layers`, src/u15-metal-ops.cc:852-855)
   if (li < m->sage_dense_layers) flags &= ~U15C_FWD_SAGE;
   const bool f8 = (flags & U15C_FWD_FP8) != 0;
-  if (i8 && f8) return fail(U15C_EINVAL, "a pass runs W8A8 or fp8, not both");
-  if (f8 && L.qkv_f8 == nullptr)
-    return fail(U15C_EINVAL, "fp8 requested but the model has no e4m3 twins "
-                             "(create with U15C_MODEL_FP8 and call u15c_model_finalize)");
   if (i8 && L.qkv8 == nullptr)
     return fail(U15C_EINVAL, "W8A8 requested but the model has no int8 twins "
                              "(create with U15C_MODEL_INT8 and call u15c_model_finalize)");
@@ -682,9 +681,24 @@ struct TpStream {
   }
 };
 
+// An fp8 pass needs twins of the projections as they are bound now. Asked
+// before a pass enqueues anything.
+int check_fp8(const u15c_model* m, unsigned flags)
+{
+  if (!(flags & U15C_FWD_FP8)) return U15C_OK;
+  if (flags & U15C_FWD_INT8) return fail(U15C_EINVAL, "a pass runs W8A8 or fp8, not both");
+  if (!(m->flags & U15C_MODEL_FP8))
+    return fail(U15C_EINVAL, "fp8 requested but the model has no e4m3 twins "
+                             "(create with U15C_MODEL_FP8 and call u15c_model_finalize)");
+  if (!m->fp8_current)
+    return fail(U15C_EINVAL, "fp8 requested but the e4m3 twins are not of the weights bound now "
+                             "(call u15c_model_finalize)");
+  return U15C_OK;
+}
+
 int validate_pass(u15c_model* m, int n, u15c_kv* kv, int kv_off, int kv_len, int attn,
                   const int32_t* pos_t, const int32_t* pos_h, const int32_t* pos_w,
-                  const int32_t* t_index)
+                  const int32_t* t_index, unsigned flags)
 {
   if (m == nullptr || kv == nullptr) return fail(U15C_EINVAL, "no model or KV cache");
   if (kv->m != m) return fail(U15C_EINVAL, "the KV cache belongs to another model");
@@ -699,7 +713,7 @@ int validate_pass(u15c_model* m, int n, u15c_kv* kv, int kv_off, int kv_len, int
   if (attn < 0 || attn > 2) return fail(U15C_EINVAL, "unknown attention rule");
   if (attn == U15C_ATTN_BLOCK_CAUSAL && t_index == nullptr)
     return fail(U15C_EINVAL, "Attn::BlockCausal needs the t-index vector");
-  return U15C_OK;
+  return check_fp8(m, flags);
 }
 
 }  // namespace
@@ -1011,6 +1025,7 @@ int u15c_model_bind(u15c_model* m, u15c_stream stream, int layer, int expert, in
     case U15C_T_FINAL_NORM: dst = m->final_norm + expert * H; whole(H); break;
     default: return fail(U15C_EINVAL, "unknown tensor id");
   }
+  const bool gains = rows == 1;   // norms have no twins
   const size_t es = dtype == U15C_DT_F32 ? 4 : 2;
   const size_t bytes = (size_t)src_rows * src_ld * es;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1026,6 +1041,7 @@ int u15c_model_bind(u15c_model* m, u15c_stream stream, int layer, int expert, in
     }
     dsrc = staging;
   }
+  if (!gains) m->fp8_current = false;
   bind_kernel<<<nblk(rows * cols, 256), 256, 0, st>>>(dsrc, dtype, rows, cols, src_ld, r0, c0,
                                                        dst, inter);
   cudaError_t e = cudaGetLastError();
@@ -1044,6 +1060,7 @@ int u15c_model_bind_random(u15c_model* m, u15c_stream stream, uint64_t seed, flo
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const u15c_config& c = m->cfg;
   const long E = c.n_experts, H = c.hidden, I = c.inter, QD = m->qd(), QKV = m->qkv_n();
+  m->fp8_current = false;
   uint64_t sid = 0;
   auto fill = [&](bf16* p, long n, float mean, float sd) {
     randn_kernel<<<nblk(n, 256), 256, 0, st>>>(p, n, seed, ++sid, mean, sd);
@@ -1086,6 +1103,7 @@ int u15c_model_finalize(u15c_model* m, u15c_stream stream)
     rc |= u15::launch_quant_rows(L.down, L.down8, L.down_s, E * H, I, st);
     if (rc) return fail(U15C_ECUDA, "finalize: quantisation launch failed");
   }
+  m->fp8_current = (m->flags & U15C_MODEL_FP8) != 0;
   return U15C_OK;
 }
 
@@ -1202,7 +1220,7 @@ int u15c_layer_forward(u15c_model* m, u15c_stream stream, int layer, void* x, in
                        int kv_off, int kv_len, const int32_t* pos_t, const int32_t* pos_h,
                        const int32_t* pos_w, int attn, const int32_t* t_index, unsigned flags)
 {
-  int rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index);
+  int rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index, flags);
   if (rc) return rc;
   if (layer < 0 || layer >= m->cfg.n_layers) return fail(U15C_EINVAL, "layer out of range");
   if (x == nullptr) return fail(U15C_EINVAL, "null activations");
@@ -1234,7 +1252,7 @@ int u15c_forward(u15c_model* m, u15c_stream stream, void* x, int n, const int* s
                  const int32_t* pos_t, const int32_t* pos_h, const int32_t* pos_w, int attn,
                  const int32_t* t_index, unsigned flags, int (*stop)(void*), void* stop_ctx)
 {
-  int rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index);
+  int rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index, flags);
   if (rc) return rc;
   if (x == nullptr) return fail(U15C_EINVAL, "null activations");
   DeviceScope ds(m->device);
@@ -1281,7 +1299,7 @@ int u15c_forward_many(u15c_model* m, u15c_stream stream, void* x, int n, const u
   for (int i = 0; i < nslots; ++i) {
     const u15c_slot& s = slots[i];
     if ((rc = validate_pass(m, n, s.kv, s.kv_off, s.kv_len, attn, s.pos_t, s.pos_h, s.pos_w,
-                            s.t_index)))
+                            s.t_index, flags)))
       return rc;
     max_kv = std::max(max_kv, s.kv_len);
   }
@@ -1344,8 +1362,8 @@ int u15c_layer_forward_host(u15c_model* m, u15c_stream stream, int layer, const 
   if (m == nullptr || x_host == nullptr || out_host == nullptr)
     return fail(U15C_EINVAL, "layer_forward_host: null argument");
   DeviceScope ds(m->device);
-  int rc = m->ensure_scratch(n, kv_len);
-  if (rc) return rc;
+  int rc = check_fp8(m, flags);
+  if (rc || (rc = m->ensure_scratch(n, kv_len))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int H = m->cfg.hidden;
   const size_t bytes = (size_t)n * H * 2;
@@ -1356,7 +1374,7 @@ int u15c_layer_forward_host(u15c_model* m, u15c_stream stream, int layer, const 
   // and tensor-parallel models take the plain upload -> layer -> download.
   constexpr int kChunks = 4;
   if (n >= 1024 && m->tp_size == 1) {
-    if ((rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index)))
+    if ((rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index, flags)))
       return rc;
     if (layer < 0 || layer >= m->cfg.n_layers) return fail(U15C_EINVAL, "layer out of range");
     u15::SegInfo seg;
@@ -1445,7 +1463,7 @@ int u15c_layer_forward_host_async(u15c_model* m, u15c_stream stream, int layer,
   if (m->tp_size != 1)
     return fail(U15C_EINVAL, "layer_forward_host_async: tensor-parallel models take the "
                              "synchronous u15c_layer_forward_host");
-  int rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index);
+  int rc = validate_pass(m, n, kv, kv_off, kv_len, attn, pos_t, pos_h, pos_w, t_index, flags);
   if (rc) return rc;
   if (layer < 0 || layer >= m->cfg.n_layers) return fail(U15C_EINVAL, "layer out of range");
   u15::SegInfo seg;
