@@ -721,9 +721,11 @@ __global__ void __launch_bounds__(kThreadsPair, 1)
 
 // ---------------------------------------------------------------------
 // Few rows: the weights are the bytes that count. A tile is 128 weight rows
-// (SwiGLU: the 128 gate rows and the 128 up rows that go with them) by MT
-// activation rows, the weights as the MMA's M = 128 side, so a lane of the
-// accumulator is an output column and its columns are the activation rows.
+// (SwiGLU: the 128 gate rows and the 128 up rows that go with them) by all the
+// activation rows there are, MT at most, the weights as the MMA's M = 128 side, so a
+// lane of the accumulator is an output column and its columns are the activation
+// rows. A segment is a unit of its own (with its expert's weights) that finishes
+// its rows of them; the rows of a pass begin at their first scale column.
 // The k-blocks of a tile are split over the CTAs of a cluster; their partial
 // sums meet in shared memory, each CTA adding (in rank order) and finishing
 // its share of the rows. The runtime keeps one CTA with a TMEM allocation on
@@ -758,10 +760,7 @@ struct FewCfg {
 
 struct FewParams {
   int N, n_kblk;
-  int nseg;
-  int seg_off[kMaxSeg + 1];
-  int seg_expert[kMaxSeg];
-  int unit_start[kMaxSeg + 1];
+  int lo[kMaxSeg], hi[kMaxSeg], expert[kMaxSeg];   // the segments that hold rows
   int sf_blk_expert;
   void* y;
   const bf16* resid;
@@ -793,14 +792,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   const uint32_t w = warp_id();
   const int split = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster is the x axis
   const int tile = blockIdx.y;
-  // the unit: an MT-row block of one segment
-  int s_ = 0;
-#pragma unroll 1
-  for (int k = 1; k < p.nseg; ++k)
-    if ((int)blockIdx.z >= p.unit_start[k]) s_ = k;
-  const int m0 = (p.seg_off[s_] / MT + ((int)blockIdx.z - p.unit_start[s_])) * MT;
-  const int lo = max(m0, p.seg_off[s_]) - m0, hi = min(m0 + MT, p.seg_off[s_ + 1]) - m0;
-  const int expert = p.seg_expert[s_];
+  const int lo = p.lo[blockIdx.z], hi = p.hi[blockIdx.z], expert = p.expert[blockIdx.z];
   // this CTA's stages of the tile, and their first k-block
   const int n_st = (p.n_kblk + C::kKps - 1) / C::kKps;
   const int st0 = rank * n_st / split, st1 = (rank + 1) * n_st / split;
@@ -821,11 +813,11 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
 #pragma unroll
         for (int h = 0; h < NA; ++h)
           tma_load_2d(st + (hk * NA + h) * kTileBytes, &tmW, (kb + hk) * 128, wrow + 128 * h, fb);
-        tma_load_2d(st + C::kKps * C::kA + hk * C::kB, &tmX, (kb + hk) * 128, m0, fb);
+        tma_load_2d(st + C::kKps * C::kA + hk * C::kB, &tmX, (kb + hk) * 128, 0, fb);
       }
       if (sfs) {
         const uint32_t sf = st + C::kKps * (C::kA + C::kB);
-        tma_load_sf(sf, &tmSX, kb >> 2, m0 >> 7, fb);
+        tma_load_sf(sf, &tmSX, kb >> 2, 0, fb);
 #pragma unroll
         for (int h = 0; h < NA; ++h)
           tma_load_sf(sf + (1 + h) * kFp8SfTile, &tmSW, kb >> 2,
@@ -932,8 +924,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
   bool ok = true;
   if (w >= 2) {
     if constexpr (EPI == kEpiResid)
-      prefetch_resid(p, m0 + lo + rank, split, m0 + hi, 128, (int)threadIdx.x - 64, tile * 128,
-                     128);
+      prefetch_resid(p, lo + rank, split, hi, 128, (int)threadIdx.x - 64, tile * 128, 128);
     // every MMA of this CTA has completed, and with them every load
     ok = warp_wait(accf, 0, p.err, kDevWaitAccFull);
     tc_fence_after();
@@ -967,7 +958,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
       constexpr int R = decltype(r_)::value, Q = decltype(q_)::value;
       for (int j0 = lo + rank + (int)w * split; j0 < hi; j0 += R * step) {
         uint2 a[R] = {};
-        addend4<EPI>(a, p, m0 + j0, step, (hi - j0 + step - 1) / step, expert, col, ncols);
+        addend4<EPI>(a, p, j0, step, (hi - j0 + step - 1) / step, expert, col, ncols);
         float4 v[Q][NA][R] = {};
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
@@ -1006,7 +997,7 @@ __global__ void __launch_bounds__(kThreadsFew, 1)
             v[2] = swiglu1(v[2], t[1][i].z);
             v[3] = swiglu1(v[3], t[1][i].w);
           }
-          finish4<EPI>(v, a[i], p, m0 + j0 + i * step, tile, col, ncols);
+          finish4<EPI>(v, a[i], p, j0 + i * step, tile, col, ncols);
         }
       }
     };
@@ -1351,13 +1342,8 @@ __global__ void __launch_bounds__(kThreadsMid, 1)
   }
 }
 
-// Row units of segment s: blocks of h rows of the whole pass, cut at the segment's
-// ends, or (pairs) blocks of 256 from its first row rounded down to 64.
-inline int few_units_of(const SegInfo& seg, int s, int h)
-{
-  const int lo = seg.off[s], hi = seg.off[s + 1];
-  return hi > lo ? (hi + h - 1) / h - lo / h : 0;
-}
+// Row units of segment s in the pair form: blocks of 256 from its first row rounded
+// down to 64.
 inline int pair_units_of(const SegInfo& seg, int s)
 {
   const int lo = seg.off[s], hi = seg.off[s + 1];
@@ -1544,7 +1530,8 @@ FewPlan few_plan_of(const GemmFp8Args& a, const SegInfo& seg, const int* residen
   constexpr bool GU = EPI == kEpiSwiglu || EPI == kEpiSwigluFp8;
   using C = FewCfg<MT, GU>;
   long tiles = 0;
-  for (int s = 0; s < seg.nseg; ++s) tiles += (long)few_tiles<EPI>(a) * few_units_of(seg, s, MT);
+  for (int s = 0; s < seg.nseg; ++s)
+    if (seg.off[s + 1] > seg.off[s]) tiles += few_tiles<EPI>(a);
   // a k-block of 128 weight rows: 160 ns; a round's set-up, first loads and
   // epilogue: 2.5 us and 20 ns a row
   const int stage_ns = C::kKps * C::kNA * 160;
@@ -1567,16 +1554,13 @@ int launch_few(const GemmFp8Args& a, const SegInfo& seg, const FewPlan& plan, cu
   p.bias = static_cast<const bf16*>(a.bias);
   p.sy = a.sy;
   p.err = a.dev_err;
-  p.nseg = seg.nseg;
-  int units = 0;
+  int units = 0;   // launch_rows: a.M <= MT
   for (int s = 0; s < seg.nseg; ++s) {
-    p.seg_off[s] = seg.off[s];
-    p.seg_expert[s] = seg.expert[s];
-    p.unit_start[s] = units;
-    units += few_units_of(seg, s, MT);
+    if (seg.off[s + 1] <= seg.off[s]) continue;
+    p.lo[units] = seg.off[s];
+    p.hi[units] = seg.off[s + 1];
+    p.expert[units++] = seg.expert[s];
   }
-  p.seg_off[seg.nseg] = seg.off[seg.nseg];
-  p.unit_start[seg.nseg] = units;
   const int tiles = few_tiles<EPI>(a);
   CUtensorMap mx, mw, msx, msw;
   const uint64_t groups = fp8_groups(a.K);
