@@ -204,11 +204,11 @@ int u15c_kv_append(u15c_stream stream, const void* in, void* pages, const int32_
 
 /* A quantised tensor is q (e4m3, one byte a value, [rows][cols] row-major)
  * and scale bytes s; it stands for q[r][c] * 2^(s[r][c / 128] - 127). s is
- * the smallest exponent for which 448 * 2^(s - 127) reaches the largest
- * magnitude of its block (0 when 2^-118 does), so no finite value saturates;
- * values are rounded to nearest even, once. A value that is not finite
- * becomes the NaN code 0x7F and makes every product with its row NaN; the
- * finite values of a block that holds an Inf become 0.
+ * the smallest exponent from 0 on for which 448 * 2^(s - 127) reaches the
+ * largest magnitude of its block (0 up to 448 * 2^-127 = 1.75 * 2^-119), so no
+ * finite value saturates; values are rounded to nearest even, once. A value
+ * that is not finite becomes the NaN code 0x7F and makes every product with
+ * its row NaN; the finite values of a block that holds an Inf become 0.
  * Blocks are 1 x 128 for activations, 128 x 128 for weights (the byte is then
  * the same for the block's 128 rows); the last block of a row or a column
  * may be short. cols must be a multiple of 16.

@@ -44,7 +44,7 @@ __host__ __device__ __forceinline__ long fp8_scale_at(long r, int b, int groups)
 
 // The scale byte of a block whose largest magnitude is amax: the smallest s
 // with amax <= 448 * 2^(s - 127), from amax's exponent field and whether its
-// mantissa is above 1.75 (448 = 1.75 * 2^8); 0 for amax below 2^-118.
+// mantissa is above 1.75 (448 = 1.75 * 2^8); 0 up to 448 * 2^-127 = 1.75 * 2^-119.
 __device__ __forceinline__ uint32_t fp8_scale_byte(float amax)
 {
   const uint32_t u = __float_as_uint(amax);
