@@ -69,11 +69,18 @@ _BYTES = (torch.uint8,)
 def _need(dev, what, t, n, dtypes):
     """The address of `t`, which must hold at least `n` values of one of `dtypes`,
     contiguous on device `dev` (the current one)."""
-    if (t.numel() < n or t.dtype not in dtypes or t.get_device() != dev
+    if (t is None or t.numel() < n or t.dtype not in dtypes or t.get_device() != dev
             or not t.is_contiguous()):
         raise L.U15Error(L.EINVAL, f"{what}: expected {n} contiguous values of "
                          f"{' or '.join(str(d) for d in dtypes)} on the current device")
     return t.data_ptr()
+
+
+def _experts(what, t):
+    """How many matrices the stack `t` holds."""
+    if t is None or t.dim() == 0:
+        raise L.U15Error(L.EINVAL, f"{what}: expected a stack of every expert's tensor")
+    return t.shape[0]
 
 
 def _need_scale(dev, what, t, rows, cols, n_experts=1):
@@ -197,7 +204,7 @@ class CudaOps:
     def mot_add_rms_norm_quant_fp8(self, x, delta, w_stack, segments, x_out, q, scale, rows, dim,
                                    eps):
         off, ex, ns = segments_arrays(segments, rows)
-        n, d, E = rows * dim, _device(), w_stack.shape[0]
+        n, d, E = rows * dim, _device(), _experts("w_stack", w_stack)
         check(lib().u15c_mot_add_rms_norm_quant_fp8(
             _raw_stream(d), _need(d, "x", x, n, _BF16),
             None if delta is None else _need(d, "delta", delta, n, _BF16),
@@ -209,7 +216,7 @@ class CudaOps:
     def mot_linear_fp8(self, xq, sx, wq_stack, sw_stack, segments, y, M, K, N,
                        epilogue=L.EPI_STORE, resid=None, bias=None):
         off, ex, ns = segments_arrays(segments, M)
-        d, E = _device(), wq_stack.shape[0]
+        d, E = _device(), _experts("wq_stack", wq_stack)
         ny = M * (N // 2 if epilogue == L.EPI_SWIGLU else N)
         check(lib().u15c_mot_linear_fp8(
             _raw_stream(d), _need(d, "xq", xq, M * K, _E4M3), _need_scale(d, "sx", sx, M, K),
@@ -221,7 +228,7 @@ class CudaOps:
 
     def mot_swiglu_fp8(self, xq, sx, wq_stack, sw_stack, segments, yq, sy, M, K, N):
         off, ex, ns = segments_arrays(segments, M)
-        d, E = _device(), wq_stack.shape[0]
+        d, E = _device(), _experts("wq_stack", wq_stack)
         check(lib().u15c_mot_swiglu_fp8(
             _raw_stream(d), _need(d, "xq", xq, M * K, _E4M3), _need_scale(d, "sx", sx, M, K),
             _need(d, "wq_stack", wq_stack, E * N * K, _E4M3),
@@ -236,7 +243,7 @@ class CudaOps:
     def mot_ffn_fp8(self, x, delta, w_norm_stack, gu, gu_scale, down, down_scale, segments, y, ws,
                     rows, hidden, inter, eps):
         off, ex, ns = segments_arrays(segments, rows)
-        d, E, n = _device(), gu.shape[0], rows * hidden
+        d, E, n = _device(), _experts("gu", gu), rows * hidden
         ws_n = lib().u15c_ffn_fp8_workspace_bytes(rows, hidden, inter)
         check(lib().u15c_mot_ffn_fp8(
             _raw_stream(d), _need(d, "x", x, n, _BF16),
