@@ -229,7 +229,7 @@ int u15c_quant_rows_fp8(u15c_stream stream, const void* x, uint8_t* q, uint8_t* 
                         int cols);
 
 /* w [n_experts][N][K] bf16 -> q, scale, one scale per 128 x 128 block of an
- * expert's matrix. */
+ * expert's matrix. At most 65535 experts of 65535 * 128 rows. */
 int u15c_quant_weight_fp8(u15c_stream stream, const void* w, uint8_t* q, uint8_t* scale,
                           int n_experts, int N, int K);
 

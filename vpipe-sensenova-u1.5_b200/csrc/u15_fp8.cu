@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, norm_ctas<NT, KW>())
   }
 }
 
-// The same for rows too wide for registers: one CTA a row, which it reads twice.
+// The same for rows too wide for registers: one CTA a row, which it reads twice
+// (4096 x 16384 without / with a residual 52.6 / 82.6 us; bytes once: 30.8 / 71.8).
 __global__ void __launch_bounds__(512)
     add_norm_wide_fp8_kernel(const bf16* x, const bf16* delta, const bf16* __restrict__ w,
                              bf16* x_out, uint8_t* __restrict__ q, uint8_t* __restrict__ scale,
